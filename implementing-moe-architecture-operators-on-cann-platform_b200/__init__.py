@@ -8,6 +8,11 @@ with the reference's names and argument meaning (op_host/moe_ops.cpp:537-679):
     expert_out          = moe_expert_ffn(x, expert_ids, weights, expert_weights)
     y                   = moe_combine(expert_out, expert_ids, weights)
 
+Next to them: moe_router_select (expert choice from router logits: softmax or sigmoid
+scores, balance bias, groups, renormalised weights), moe_linear (a matrix product with
+bias, activation, gate and residual in its epilogue) and moe_shared_layer_forward (the
+layer with such a router and a shared expert).
+
 There is no CPU fallback: if the library is missing, or a tensor is not on a
 CUDA device, the call raises.
 """
@@ -20,8 +25,12 @@ from .ops import (  # noqa: F401
     moe_expert_ffn_workspace_size,
     moe_layer_forward,
     moe_layer_workspace_size,
+    moe_linear,
     moe_permute,
+    moe_router_select,
     moe_routing_topk,
+    moe_shared_layer_forward,
+    moe_shared_layer_workspace_size,
     device_error,
     infer_shapes,
     trace_start,
@@ -35,7 +44,8 @@ from .inputs import make_inputs, make_inputs_torch, CONFIGS  # noqa: F401
 
 
 def register_torch_ops():
-    """Registers torch.ops.moe_b200.* (routing_topk, expert_ffn, combine, layer_forward)."""
+    """Registers torch.ops.moe_b200.* (routing_topk, expert_ffn, combine, layer_forward,
+    router_select, linear)."""
     from . import torch_ops  # noqa: F401
 
     return torch_ops

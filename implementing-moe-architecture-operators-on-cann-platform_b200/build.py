@@ -14,7 +14,8 @@ CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libmoe_b200.so")
 
-SOURCES = ["routing.cu", "permute.cu", "grouped_gemm.cu", "combine.cu", "moe_ops.cu", "no_alloc.cu", "ep.cu"]
+SOURCES = ["routing.cu", "permute.cu", "grouped_gemm.cu", "combine.cu", "moe_ops.cu", "no_alloc.cu", "ep.cu",
+           "select.cu", "linear.cu"]
 HEADERS = ["moe_common.cuh", "moe_kernels.h"]
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")

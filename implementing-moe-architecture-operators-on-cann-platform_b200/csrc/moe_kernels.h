@@ -99,4 +99,33 @@ cudaError_t launch_gemm_down_ptr(const __half* h, const __half* expert_weights, 
 cudaError_t launch_combine(const __half* expert_out, const __half* weights, __half* y, int T,
                            int H, int K, cudaStream_t s);
 
+// ---- MoeRouterSelect (select.cu)
+struct SelectArgs {
+    const void* logits;   // [T, E], rows ldl elements apart
+    const float* bias;    // [E] or nullptr
+    int32_t* ids;         // [T, K]
+    void* weights;        // [T, K], type wtype
+    long long ldl;
+    int T, E, K;
+    int G, topG, groupTop;
+    int wtype;            // MOE_DT_FLOAT or MOE_DT_FLOAT16
+    int sigmoid, renorm;
+    float scale;
+};
+cudaError_t launch_select(const SelectArgs& a, int ltype, cudaStream_t s);
+
+// ---- MoeLinear (linear.cu)
+struct LinearArgs {
+    const void* x;         // [T, K], rows ldx elements apart
+    const void* w;         // [N, K] ([2N, K] when gated), rows ldw elements apart
+    const void* bias;      // [N] ([2N]) or nullptr, the type of x
+    const void* residual;  // [T, N] or nullptr, rows ldr elements apart, the type of y
+    void* y;               // [T, N], rows ldy elements apart
+    long long ldx, ldw, ldr, ldy;
+    int T, K, N;
+    int type, otype;       // MOE_DT_* of x/w/bias and of y/residual
+    int act, gated;
+};
+cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s);
+
 }  // namespace moe

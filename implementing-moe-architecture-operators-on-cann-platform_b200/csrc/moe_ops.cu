@@ -193,6 +193,115 @@ int run_ffn(const void* x, const int32_t* ids, const void* ew, void* out, int64_
     return cuda_status(e);
 }
 
+inline bool is_aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+inline size_t dtype_size(int t) { return t == MOE_DT_FLOAT ? 4 : 2; }
+
+// Checks of MoeRouterSelect; fills the kernel's arguments.
+int select_args(moe::SelectArgs& a, const void* logits, int logitsDtype, int64_t ldl, const float* bias,
+                int32_t* ids, void* weights, int weightsDtype, int64_t T, int64_t E, int64_t K, int64_t G,
+                int64_t topG, int groupTop, int scoreFunc, int renormalize, float scale)
+{
+    if (T < 0 || E < 1 || E > 256 || K < 1 || K > 8 || T * K >= (int64_t(1) << 31)) return MOE_ERR_BAD_SHAPE;
+    if (G < 1 || G > 32 || E % G || topG < 1 || topG > G || K > topG * (E / G)) return MOE_ERR_BAD_SHAPE;
+    if (groupTop < 1 || groupTop > 2 || (groupTop == 2 && E / G < 2)) return MOE_ERR_BAD_SHAPE;
+    if (ldl == 0) ldl = E;
+    if (ldl < E || ldl > (int64_t(1) << 32)) return MOE_ERR_BAD_SHAPE;
+    if (logitsDtype != MOE_DT_FLOAT && logitsDtype != MOE_DT_FLOAT16 && logitsDtype != MOE_DT_BF16)
+        return MOE_ERR_UNSUPPORTED;
+    if (weightsDtype != MOE_DT_FLOAT && weightsDtype != MOE_DT_FLOAT16) return MOE_ERR_UNSUPPORTED;
+    if (scoreFunc != MOE_SCORE_SOFTMAX && scoreFunc != MOE_SCORE_SIGMOID) return MOE_ERR_UNSUPPORTED;
+    if (T > 0 && (!logits || !ids || !weights)) return MOE_ERR_NULL_POINTER;
+    if (!is_aligned(logits, dtype_size(logitsDtype)) || !is_aligned(bias, 4) || !is_aligned(ids, 4) ||
+        !is_aligned(weights, dtype_size(weightsDtype)))
+        return MOE_ERR_MISALIGNED;
+    a.logits = logits;
+    a.bias = bias;
+    a.ids = ids;
+    a.weights = weights;
+    a.ldl = ldl;
+    a.T = (int)T;
+    a.E = (int)E;
+    a.K = (int)K;
+    a.G = (int)G;
+    a.topG = (int)topG;
+    a.groupTop = groupTop;
+    a.wtype = weightsDtype;
+    a.sigmoid = scoreFunc == MOE_SCORE_SIGMOID;
+    a.renorm = renormalize != 0;
+    a.scale = scale;
+    return MOE_OK;
+}
+
+// Checks of MoeLinear; fills the kernel's arguments.
+int linear_args(moe::LinearArgs& a, const void* x, const void* w, const void* bias, const void* residual, void* y,
+                int64_t T, int64_t K, int64_t N, int64_t ldx, int64_t ldw, int64_t ldr, int64_t ldy, int dtype,
+                int outDtype, int activation, int gated)
+{
+    const int64_t lim = int64_t(1) << 30;  // rows, features; twice of it still fits an int32
+    if (T < 0 || T > lim || K < 8 || (K & 7) || K > lim || N < 1 || N > lim) return MOE_ERR_BAD_SHAPE;
+    if (dtype != MOE_DT_FLOAT16 && dtype != MOE_DT_BF16) return MOE_ERR_UNSUPPORTED;
+    if (outDtype != dtype && outDtype != MOE_DT_FLOAT) return MOE_ERR_UNSUPPORTED;
+    if (activation < MOE_ACT_NONE || activation > MOE_ACT_SIGMOID) return MOE_ERR_UNSUPPORTED;
+    if (ldx == 0) ldx = K;
+    if (ldw == 0) ldw = K;
+    if (ldr == 0) ldr = N;
+    if (ldy == 0) ldy = N;
+    const int64_t ldlim = int64_t(1) << 36;  // a tensor map's row pitch is below 2^40 bytes
+    if (ldx < K || ldw < K || ldr < N || ldy < N || ldx > ldlim || ldw > ldlim || ldr > ldlim || ldy > ldlim)
+        return MOE_ERR_BAD_SHAPE;
+    if (residual && residual == y && ldr != ldy) return MOE_ERR_BAD_SHAPE;
+    if (T > 0 && (!x || !w || !y)) return MOE_ERR_NULL_POINTER;
+    if (!aligned16(x) || !aligned16(w) || (ldx & 7) || (ldw & 7)) return MOE_ERR_MISALIGNED;
+    if (!is_aligned(bias, dtype_size(dtype)) || !is_aligned(residual, dtype_size(outDtype)) ||
+        !is_aligned(y, dtype_size(outDtype)))
+        return MOE_ERR_MISALIGNED;
+    a.x = x;
+    a.w = w;
+    a.bias = bias;
+    a.residual = residual;
+    a.y = y;
+    a.ldx = ldx;
+    a.ldw = ldw;
+    a.ldr = ldr;
+    a.ldy = ldy;
+    a.T = (int)T;
+    a.K = (int)K;
+    a.N = (int)N;
+    a.type = dtype;
+    a.otype = outDtype;
+    a.act = activation;
+    a.gated = gated != 0;
+    return MOE_OK;
+}
+
+int run_linear(const moe::LinearArgs& a, cudaStream_t s)
+{
+    cudaError_t e = moe::launch_linear(a, s);
+    if (e == cudaErrorInvalidValue) return MOE_ERR_UNSUPPORTED;  // tensor map rejected
+    return cuda_status(e);
+}
+
+struct SharedLayout {
+    LayerLayout l;
+    size_t logits, hs, total;
+};
+
+SharedLayout shared_layout(int64_t T, int64_t H, int64_t E, int64_t K, int64_t I, int64_t Is)
+{
+    SharedLayout L;
+    L.l = layer_layout(T, H, E, K, I);
+    size_t o = L.l.total;
+    const size_t t = (size_t)(T > 0 ? T : 1);
+    L.logits = o;
+    o += align_up(t * (size_t)E * 4);
+    L.hs = o;
+    o += align_up(t * (size_t)(Is > 0 ? Is : 1) * 2);
+    L.total = o;
+    return L;
+}
+
+bool shared_size_ok(int64_t Is) { return Is >= 0 && !(Is & 7) && Is <= (int64_t(1) << 30); }
+
 }  // namespace
 
 extern "C" {
@@ -297,6 +406,85 @@ int MoeLayerForward(const void* x, const void* w_gate, const void* expert_weight
     rc = cuda_status(moe::launch_combine(static_cast<const __half*>(expert_out),
                                          static_cast<const __half*>(weights),
                                          static_cast<__half*>(y), (int)T, (int)H, (int)K, s));
+    trace_mark(ev, 6, s);
+    return rc;
+}
+
+int MoeRouterSelect(const void* logits, int logitsDtype, int64_t ldl, const float* bias, int32_t* expert_ids,
+                    void* weights, int weightsDtype, int64_t T, int64_t E, int64_t K, int64_t G, int64_t topG,
+                    int groupTop, int scoreFunc, int renormalize, float scale, void* stream)
+{
+    moe::SelectArgs a;
+    int rc = select_args(a, logits, logitsDtype, ldl, bias, expert_ids, weights, weightsDtype, T, E, K, G, topG,
+                         groupTop, scoreFunc, renormalize, scale);
+    if (rc != MOE_OK || T == 0) return rc;
+    return cuda_status(moe::launch_select(a, logitsDtype, static_cast<cudaStream_t>(stream)));
+}
+
+int MoeLinear(const void* x, const void* weight, const void* bias, const void* residual, void* y, int64_t T,
+              int64_t K, int64_t N, int64_t ldx, int64_t ldw, int64_t ldr, int64_t ldy, int dtype, int outDtype,
+              int activation, int gated, void* stream)
+{
+    moe::LinearArgs a;
+    int rc = linear_args(a, x, weight, bias, residual, y, T, K, N, ldx, ldw, ldr, ldy, dtype, outDtype, activation,
+                         gated);
+    if (rc != MOE_OK || T == 0) return rc;
+    return run_linear(a, static_cast<cudaStream_t>(stream));
+}
+
+size_t MoeSharedLayerWorkspaceSize(int64_t T, int64_t H, int64_t E, int64_t K, int64_t I, int64_t Is)
+{
+    if (!ffn_shapes_ok(T, H, E, K, I) || !shared_size_ok(Is)) return 0;
+    return shared_layout(T, H, E, K, I, Is).total;
+}
+
+int MoeSharedLayerForward(const void* x, const void* w_router, const float* router_bias, const void* expert_weights,
+                          const void* shared_gate_up, const void* shared_down, void* y, int32_t* expert_ids,
+                          void* weights, int64_t T, int64_t H, int64_t E, int64_t K, int64_t I, int64_t Is, int64_t G,
+                          int64_t topG, int groupTop, int scoreFunc, int renormalize, float scale, void* workspace,
+                          size_t ws_bytes, void* stream)
+{
+    if (!ffn_shapes_ok(T, H, E, K, I) || !shared_size_ok(Is)) return MOE_ERR_BAD_SHAPE;
+    if (!workspace) return MOE_ERR_NULL_POINTER;
+    const SharedLayout L = shared_layout(T, H, E, K, I, Is);
+    if (ws_bytes < L.total) return MOE_ERR_WORKSPACE_TOO_SMALL;
+    if (T > 0 && (!x || !w_router || !expert_weights || !y || (Is > 0 && (!shared_gate_up || !shared_down))))
+        return MOE_ERR_NULL_POINTER;
+    if (!aligned16(workspace) || (T > 0 && (!aligned16(expert_weights) || !aligned16(y)))) return MOE_ERR_MISALIGNED;
+    if (!expert_ids) expert_ids = at<int32_t>(workspace, L.l.ids);
+    if (!weights) weights = at<void>(workspace, L.l.weights);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    // every argument is checked before the first launch
+    moe::LinearArgs gate, up, down;
+    moe::SelectArgs sel;
+    float* logits = at<float>(workspace, L.logits);
+    void* hs = at<void>(workspace, L.hs);
+    int rc = linear_args(gate, x, w_router, nullptr, nullptr, logits, T, H, E, 0, 0, 0, 0, MOE_DT_FLOAT16,
+                         MOE_DT_FLOAT, MOE_ACT_NONE, 0);
+    if (rc == MOE_OK)
+        rc = select_args(sel, logits, MOE_DT_FLOAT, 0, router_bias, expert_ids, weights, MOE_DT_FLOAT16, T, E, K, G,
+                         topG, groupTop, scoreFunc, renormalize, scale);
+    if (rc == MOE_OK && Is > 0)
+        rc = linear_args(up, x, shared_gate_up, nullptr, nullptr, hs, T, H, Is, 0, 0, 0, 0, MOE_DT_FLOAT16,
+                         MOE_DT_FLOAT16, MOE_ACT_SILU, 1);
+    if (rc == MOE_OK && Is > 0)
+        rc = linear_args(down, hs, shared_down, nullptr, y, y, T, Is, H, 0, 0, 0, 0, MOE_DT_FLOAT16, MOE_DT_FLOAT16,
+                         MOE_ACT_NONE, 0);
+    if (rc != MOE_OK) return rc;
+    void* expert_out = at<void>(workspace, L.l.expert_out);
+    if (T == 0) return run_ffn(x, expert_ids, expert_weights, expert_out, T, H, E, K, I, workspace, L.l.f, s, nullptr);
+    cudaEvent_t* ev = trace_begin_call();
+    trace_mark(ev, 0, s);
+    rc = run_linear(gate, s);
+    if (rc == MOE_OK) rc = cuda_status(moe::launch_select(sel, MOE_DT_FLOAT, s));
+    if (rc != MOE_OK) return rc;
+    trace_mark(ev, 1, s);
+    rc = run_ffn(x, expert_ids, expert_weights, expert_out, T, H, E, K, I, workspace, L.l.f, s, ev);
+    if (rc != MOE_OK) return rc;
+    rc = cuda_status(moe::launch_combine(static_cast<const __half*>(expert_out), static_cast<const __half*>(weights),
+                                         static_cast<__half*>(y), (int)T, (int)H, (int)K, s));
+    if (rc == MOE_OK && Is > 0) rc = run_linear(up, s);
+    if (rc == MOE_OK && Is > 0) rc = run_linear(down, s);
     trace_mark(ev, 6, s);
     return rc;
 }

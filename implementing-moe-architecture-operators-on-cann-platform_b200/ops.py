@@ -74,6 +74,13 @@ def lib():
         L.MoePermuteWorkspaceSize.argtypes = [_i64] * 3
         L.MoePermuteWorkspaceSize.restype = _sz
         L.MoePermute.argtypes = [_vp] * 3 + [_i64] * 3 + [_vp, _sz, _vp]
+        _int = ctypes.c_int
+        L.MoeRouterSelect.argtypes = [_vp, _int, _i64, _vp, _vp, _vp, _int] + [_i64] * 5 + [
+            _int, _int, _int, ctypes.c_float, _vp]
+        L.MoeLinear.argtypes = [_vp] * 5 + [_i64] * 7 + [_int] * 4 + [_vp]
+        L.MoeSharedLayerWorkspaceSize.argtypes = [_i64] * 6
+        L.MoeSharedLayerWorkspaceSize.restype = _sz
+        L.MoeSharedLayerForward.argtypes = [_vp] * 9 + [_i64] * 8 + [_int] * 3 + [ctypes.c_float, _vp, _sz, _vp]
         L.MoeGetDeviceError.argtypes = [_vp, _intp, _vp]
         L.MoeStatusString.argtypes = [ctypes.c_int]
         L.MoeStatusString.restype = ctypes.c_char_p
@@ -217,6 +224,202 @@ def moe_layer_forward(x, w_gate, expert_weights, topK: int = 2, y=None, expert_i
     _check(lib().MoeLayerForward(_ptr(x), _ptr(w_gate), _ptr(expert_weights), _ptr(y), _ptr(expert_ids),
                                  _ptr(weights), _ptr(expert_out), T, H, E, K, I, _ptr(workspace),
                                  workspace.numel(), _stream_handle(x)), "MoeLayerForward")
+    return y
+
+
+# ----------------------------------------------------------------------------- router selection, linear
+SCORE_FUNCS = {"softmax": 0, "sigmoid": 1}
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4, "sigmoid": 5}
+
+
+def _dtype_codes():
+    """torch dtype -> MOE_DT_* code (include/moe_ops.h)."""
+    global _codes
+    if _codes is None:
+        torch = _torch()
+        _codes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 27}
+    return _codes
+
+
+_codes = None
+
+
+def _rows(t, name, rows, cols, dtype, like):
+    """The row stride of a [rows, cols] CUDA matrix whose rows are contiguous (0 for a
+    single row); raises MoeError on anything else."""
+    if t.device != like.device:
+        raise MoeError(-1, f"{name} must be on {like.device} (no CPU fallback), got {t.device}")
+    if t.dtype != dtype:
+        raise MoeError(-2, f"{name} must be {dtype}, got {t.dtype}")
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
+        raise MoeError(-2, f"{name} must be [{rows}, {cols}], got {list(t.shape)}")
+    if t.is_contiguous():
+        return cols
+    if cols > 1 and t.stride(1) != 1:
+        raise MoeError(-2, f"{name}: the elements of a row must be contiguous")
+    if rows <= 1:
+        return cols
+    if t.stride(0) < cols:
+        raise MoeError(-2, f"{name}: rows must not overlap")
+    return t.stride(0)
+
+
+def _vector(t, name, n, dtype, like):
+    if t.device != like.device:
+        raise MoeError(-1, f"{name} must be on {like.device} (no CPU fallback), got {t.device}")
+    if t.dtype != dtype:
+        raise MoeError(-2, f"{name} must be {dtype}, got {t.dtype}")
+    if t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise MoeError(-2, f"{name} must be a contiguous [{n}], got {list(t.shape)}")
+
+
+def _call_on(device, fn, *args):
+    """fn(*args, stream) with `device` current: a kernel goes to its tensors' device, on
+    that device's current stream."""
+    torch = _torch()
+    if device.index == torch.cuda.current_device():
+        return fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    with torch.cuda.device(device):
+        return fn(*args, torch.cuda.current_stream(device).cuda_stream)
+
+
+def moe_router_select(logits, topK: int = 2, bias=None, numGroups: int = 1, topGroups: int = 1, groupTop: int = 1,
+                      scoreFunc: str = "softmax", renormalize: bool = False, scale: float = 1.0, expert_ids=None,
+                      weights=None):
+    """logits [T,E] (fp32, fp16 or bf16) -> (expert_ids [T,K] int32, weights [T,K] fp16).
+
+    Scores are a softmax or a sigmoid of the logits; `bias` [E] fp32 steers the choice and
+    not the weight; the choice is made inside the `topGroups` best of `numGroups` groups
+    (a group is worth its largest key, or its two largest with groupTop=2); weights are
+    renormalised over the K chosen and scaled on request.  `weights` may be a preallocated
+    fp16 or fp32 tensor.  Rows of `logits` may be padded (any row stride)."""
+    torch = _torch()
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
+        raise MoeError(-1, "logits must be a CUDA tensor (no CPU fallback)")
+    lt = _dtype_codes().get(logits.dtype)
+    if lt is None or logits.dim() != 2:
+        raise MoeError(-2, "logits must be a [T, E] matrix of float32, float16 or bfloat16")
+    if scoreFunc not in SCORE_FUNCS:
+        raise MoeError(-5, f"scoreFunc {scoreFunc!r}")
+    T, E = logits.shape
+    K = topK if topK > 0 else 2
+    ldl = _rows(logits, "logits", T, E, logits.dtype, logits)
+    if bias is not None:
+        _vector(bias, "bias", E, torch.float32, logits)
+    if expert_ids is None:
+        expert_ids = torch.empty((T, K), dtype=torch.int32, device=logits.device)
+    elif _rows(expert_ids, "expert_ids", T, K, torch.int32, logits) != K:
+        raise MoeError(-2, "expert_ids must be contiguous")
+    if weights is None:
+        weights = torch.empty((T, K), dtype=torch.float16, device=logits.device)
+    elif _rows(weights, "weights", T, K, torch.float32 if weights.dtype == torch.float32 else torch.float16,
+               logits) != K:
+        raise MoeError(-2, "weights must be contiguous")
+    _check(_call_on(logits.device, lib().MoeRouterSelect, logits.data_ptr(), lt, ldl,
+                    None if bias is None else bias.data_ptr(), expert_ids.data_ptr(), weights.data_ptr(),
+                    0 if weights.dtype == torch.float32 else 1, T, E, K, numGroups, topGroups, groupTop,
+                    SCORE_FUNCS[scoreFunc], renormalize, scale), "MoeRouterSelect")
+    return expert_ids, weights
+
+
+def moe_linear(x, weight, bias=None, activation: str = "none", gated: bool = False, residual=None, y=None,
+               out_dtype=None):
+    """x [T,K], weight [N,K] (fp16 or bf16) -> y [T,N] = act(x weight^T + bias) + residual.
+
+    gated: weight [2N,K] and bias [2N] hold the gate's rows, then the up projection's, and
+    y = act(gate) * up + residual.  y has x's dtype, or float32 (out_dtype, or the dtype of
+    a given y); residual has y's dtype and may be y itself.  Rows of every matrix may be
+    padded; K and the row strides of x and weight are multiples of 8."""
+    torch = _torch()
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise MoeError(-1, "x must be a CUDA tensor (no CPU fallback)")
+    codes = _dtype_codes()
+    dt = x.dtype
+    if dt not in codes or dt == torch.float32 or x.dim() != 2:
+        raise MoeError(-2, "x must be a [T, K] matrix of float16 or bfloat16")
+    if activation not in ACTIVATIONS:
+        raise MoeError(-5, f"activation {activation!r}")
+    if weight.dim() != 2 or (gated and weight.shape[0] & 1):
+        raise MoeError(-2, "weight must be [N, K], or [2N, K] when gated")
+    T, K = x.shape
+    rows = weight.shape[0]
+    N = rows // 2 if gated else rows
+    ldx = _rows(x, "x", T, K, dt, x)
+    ldw = _rows(weight, "weight", rows, K, dt, x)
+    if bias is not None:
+        _vector(bias, "bias", rows, dt, x)
+    if y is None:
+        ot = out_dtype if out_dtype is not None else (residual.dtype if residual is not None else dt)
+        y = torch.empty((T, N), dtype=ot, device=x.device)
+    else:
+        ot = y.dtype
+        if out_dtype is not None and out_dtype != ot:
+            raise MoeError(-2, f"y must be {out_dtype}, got {ot}")
+    if ot not in codes:
+        raise MoeError(-5, f"y of {ot}")
+    ldy = _rows(y, "y", T, N, ot, x)
+    ldr = _rows(residual, "residual", T, N, ot, x) if residual is not None else 0
+    _check(_call_on(x.device, lib().MoeLinear, x.data_ptr(), weight.data_ptr(),
+                    None if bias is None else bias.data_ptr(), None if residual is None else residual.data_ptr(),
+                    y.data_ptr(), T, K, N, ldx, ldw, ldr, ldy, codes[dt], codes[ot], ACTIVATIONS[activation],
+                    gated), "MoeLinear")
+    return y
+
+
+def moe_shared_layer_workspace_size(T, H, E, K, I, Is) -> int:
+    return int(lib().MoeSharedLayerWorkspaceSize(T, H, E, K, I, Is))
+
+
+def moe_shared_layer_forward(x, w_router, expert_weights, shared_gate_up=None, shared_down=None, topK: int = 2,
+                             router_bias=None, numGroups: int = 1, topGroups: int = 1, groupTop: int = 1,
+                             scoreFunc: str = "softmax", renormalize: bool = False, scale: float = 1.0, y=None,
+                             expert_ids=None, weights=None, workspace=None):
+    """Gate -> moe_router_select -> expert FFN -> combine, plus a shared expert over every
+    token; returns y [T,H] fp16.
+
+    x [T,H], w_router [E,H], expert_weights [E,3I,H], shared_gate_up [2Is,H] and
+    shared_down [H,Is] (both or neither), all contiguous fp16; router_bias [E] fp32."""
+    torch = _torch()
+    f16 = torch.float16
+    for t, name in ((x, "x"), (w_router, "w_router"), (expert_weights, "expert_weights")):
+        _cuda(t, name, f16)
+    if x.dim() != 2 or w_router.dim() != 2 or expert_weights.dim() != 3:
+        raise MoeError(-2, "MoeSharedLayerForward shapes")
+    T, H = x.shape
+    E = w_router.shape[0]
+    I = expert_weights.shape[1] // 3
+    K = topK if topK > 0 else 2
+    if scoreFunc not in SCORE_FUNCS:
+        raise MoeError(-5, f"scoreFunc {scoreFunc!r}")
+    if (shared_gate_up is None) != (shared_down is None):
+        raise MoeError(-2, "shared_gate_up and shared_down go together")
+    Is = 0 if shared_down is None else shared_down.shape[-1]
+    shapes = [(w_router, "w_router", (E, H)), (expert_weights, "expert_weights", (E, 3 * I, H))]
+    if Is:
+        shapes += [(shared_gate_up, "shared_gate_up", (2 * Is, H)), (shared_down, "shared_down", (H, Is))]
+    if y is not None:
+        shapes.append((y, "y", (T, H)))
+    if weights is not None:
+        shapes.append((weights, "weights", (T, K)))
+    for t, name, shape in shapes:
+        _cuda(t, name, f16)
+        if tuple(t.shape) != shape or t.device != x.device:
+            raise MoeError(-2, f"{name} must be {list(shape)} on {x.device}, got {list(t.shape)} on {t.device}")
+    if expert_ids is not None:
+        _cuda(expert_ids, "expert_ids", torch.int32)
+        if tuple(expert_ids.shape) != (T, K) or expert_ids.device != x.device:
+            raise MoeError(-2, f"expert_ids must be [{T}, {K}] on {x.device}")
+    if router_bias is not None:
+        _vector(router_bias, "router_bias", E, torch.float32, x)
+    if y is None:
+        y = torch.empty((T, H), dtype=f16, device=x.device)
+    if workspace is None:
+        workspace = _workspace(moe_shared_layer_workspace_size(T, H, E, K, I, Is), x.device)
+    _check(_call_on(x.device, lib().MoeSharedLayerForward, _ptr(x), _ptr(w_router), _ptr(router_bias),
+                    _ptr(expert_weights), _ptr(shared_gate_up), _ptr(shared_down), _ptr(y), _ptr(expert_ids),
+                    _ptr(weights), T, H, E, K, I, Is, numGroups, topGroups, groupTop, SCORE_FUNCS[scoreFunc],
+                    int(bool(renormalize)), float(scale), _ptr(workspace), workspace.numel()),
+           "MoeSharedLayerForward")
     return y
 
 

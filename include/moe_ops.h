@@ -51,9 +51,12 @@ extern "C" {
 #define MOE_ERR_TIMEOUT (-8)
 #define MOE_ERR_DEVICE (-9)
 
-/* Data-type codes of the shape/dtype inference mirror (ge::DataType values). */
+/* Data-type codes (ge::DataType values): the shape/dtype inference mirror, and the
+ * type arguments of MoeRouterSelect and MoeLinear. */
+#define MOE_DT_FLOAT 0
 #define MOE_DT_FLOAT16 1
 #define MOE_DT_INT32 3
+#define MOE_DT_BF16 27
 
 /* ------------------------------------------------------------------ operators */
 
@@ -118,6 +121,79 @@ int MoeLayerForward(const void* x, const void* w_gate, const void* expert_weight
                     int64_t hiddenSize, int64_t numExperts, int64_t topK,
                     int64_t intermediateSize, void* workspace, size_t workspaceBytes,
                     void* stream);
+
+/* ------------------------------------------------------------------ router selection
+ * Expert choice from given router logits, for routers that MoeRoutingTopK's plain
+ * softmax does not cover (no counterpart in the reference).  Per token:
+ *   score  s = softmax(logits) or 1 / (1 + exp(-logits));
+ *   key    s + bias (bias [numExperts] fp32, may be NULL): steers the choice only;
+ *   groups numGroups consecutive groups of numExperts / numGroups experts; a group's
+ *          value is its largest key (groupTop 1) or the sum of its two largest
+ *          (groupTop 2); the topGroups best groups stay, ties to the lower group;
+ *   ids    the topK largest keys, larger first, ties to the lower id;
+ *   weight s of the chosen expert, divided by the sum over the topK when renormalize
+ *          is nonzero, times scale.
+ * The choice is exact: keys that differ in 64-bit arithmetic are told apart (without a
+ * bias, logits that differ at all).  An expert whose logit or bias is -inf or NaN, or
+ * whose group did not stay, is closed: it is chosen only when no open expert is left,
+ * lowest id first, and then has weight 0.  A +inf logit has score 1 (softmax: +inf
+ * logits share it).
+ * logits [T, numExperts], rows ldLogits elements apart (0: numExperts), of type
+ * MOE_DT_FLOAT, MOE_DT_FLOAT16 or MOE_DT_BF16; expert_ids [T, topK]; weights [T, topK]
+ * of type MOE_DT_FLOAT16 (what MoeCombine takes) or MOE_DT_FLOAT.
+ * numExperts in [1,256], topK in [1, min(8, topGroups * numExperts / numGroups)],
+ * numGroups in [1,32] and a divisor of numExperts, topGroups in [1,numGroups],
+ * groupTop 1 or 2 (2 needs groups of at least 2).  numTokens == 0 is a no-op. */
+#define MOE_SCORE_SOFTMAX 0
+#define MOE_SCORE_SIGMOID 1
+int MoeRouterSelect(const void* logits, int logitsDtype, int64_t ldLogits, const float* bias,
+                    int32_t* expert_ids, void* weights, int weightsDtype, int64_t numTokens,
+                    int64_t numExperts, int64_t topK, int64_t numGroups, int64_t topGroups,
+                    int groupTop, int scoreFunc, int renormalize, float scale, void* stream);
+
+/* ------------------------------------------------------------------ linear
+ * A matrix product with its epilogue: a router's gate, the projections of a shared
+ * expert (no counterpart in the reference).
+ *   gated == 0: y = act(x W^T + bias) + residual,       W [N, K], bias [N]
+ *   gated != 0: y = act(x Wg^T + bg) * (x Wu^T + bu) + residual, W = Wg [N, K] then
+ *               Wu [N, K], bias = bg [N] then bu [N]
+ * x [T, K], W and bias have the type dtype (MOE_DT_FLOAT16 or MOE_DT_BF16); y [T, N]
+ * and residual [T, N] the type outDtype (dtype, or MOE_DT_FLOAT).  bias and residual
+ * may be NULL.  Sums and the epilogue are fp32; y is rounded once.  ldx, ldw, ldr, ldy:
+ * elements from one row to the next (0: contiguous).  K, ldx and ldw are multiples of
+ * 8 and x and W 16-byte aligned; N, ldr, ldy and the other pointers are free (best when
+ * 16-byte aligned too).  residual may be y itself (same rows); y overlaps no other
+ * input.  numTokens == 0 is a no-op. */
+#define MOE_ACT_NONE 0
+#define MOE_ACT_RELU 1
+#define MOE_ACT_GELU 2       /* z * Phi(z) */
+#define MOE_ACT_GELU_TANH 3  /* its tanh form */
+#define MOE_ACT_SILU 4
+#define MOE_ACT_SIGMOID 5
+int MoeLinear(const void* x, const void* weight, const void* bias, const void* residual, void* y,
+              int64_t numTokens, int64_t inFeatures, int64_t outFeatures, int64_t ldx, int64_t ldw,
+              int64_t ldr, int64_t ldy, int dtype, int outDtype, int activation, int gated,
+              void* stream);
+
+/* ------------------------------------------------------------------ layer with a shared expert
+ * The whole layer with a selecting router and an optional shared expert:
+ *   logits = x w_router^T (fp32), MoeRouterSelect, MoeExpertFFN, MoeCombine, then
+ *   y += (silu(x Sg^T) * (x Su^T)) Sd^T over every token.
+ * x [T,H], w_router [E,H], expert_weights [E,3I,H], shared_gate_up [2*Is,H] (Sg then
+ * Su), shared_down [H,Is], y [T,H], all fp16; router_bias [E] fp32 or NULL; Is ==
+ * sharedSize, a multiple of 8, or 0 without a shared expert (its weights are then NULL).
+ * expert_ids [T,K] / weights [T,K] fp16 receive the choice, or are NULL.  The other
+ * arguments are MoeRouterSelect's.  The workspace's first word is the device error
+ * word (MoeGetDeviceError). */
+size_t MoeSharedLayerWorkspaceSize(int64_t numTokens, int64_t hiddenSize, int64_t numExperts,
+                                   int64_t topK, int64_t intermediateSize, int64_t sharedSize);
+int MoeSharedLayerForward(const void* x, const void* w_router, const float* router_bias,
+                          const void* expert_weights, const void* shared_gate_up,
+                          const void* shared_down, void* y, int32_t* expert_ids, void* weights,
+                          int64_t numTokens, int64_t hiddenSize, int64_t numExperts, int64_t topK,
+                          int64_t intermediateSize, int64_t sharedSize, int64_t numGroups,
+                          int64_t topGroups, int groupTop, int scoreFunc, int renormalize,
+                          float scale, void* workspace, size_t workspaceBytes, void* stream);
 
 /* ------------------------------------------------------------------ expert parallel
  * The layer partitioned expert-parallel over n GPUs (one process or thread per
