@@ -125,7 +125,11 @@ struct LinearArgs {
     int T, K, N;
     int type, otype;       // MOE_DT_* of x/w/bias and of y/residual
     int act, gated;
+    int* err;              // error word of its bounded waits; nullptr: the library's own
 };
+// Device address of the linear kernels' error word on the current device (their calls
+// have no workspace); nullptr if the lookup fails.
+int* linear_error_word();
 cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s);
 
 }  // namespace moe

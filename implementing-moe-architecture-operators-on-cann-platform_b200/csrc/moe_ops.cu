@@ -271,6 +271,7 @@ int linear_args(moe::LinearArgs& a, const void* x, const void* w, const void* bi
     a.otype = outDtype;
     a.act = activation;
     a.gated = gated != 0;
+    a.err = nullptr;
     return MOE_OK;
 }
 
@@ -279,6 +280,22 @@ int run_linear(const moe::LinearArgs& a, cudaStream_t s)
     cudaError_t e = moe::launch_linear(a, s);
     if (e == cudaErrorInvalidValue) return MOE_ERR_UNSUPPORTED;  // tensor map rejected
     return cuda_status(e);
+}
+
+// Synchronises `stream`, copies a per-device error word to *code and clears it.
+int take_error_word(int* (*find)(), int* code, void* stream)
+{
+    if (!code) return MOE_ERR_NULL_POINTER;
+    int* word = find();
+    if (!word) return cuda_status(cudaErrorInvalidSymbol);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    int v = 0;
+    cudaError_t e = cudaMemcpyAsync(&v, word, sizeof(int), cudaMemcpyDeviceToHost, s);
+    if (e == cudaSuccess) e = cudaMemsetAsync(word, 0, sizeof(int), s);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+    if (e != cudaSuccess) return cuda_status(e);
+    *code = v;
+    return MOE_OK;
 }
 
 struct SharedLayout {
@@ -479,7 +496,10 @@ int MoeSharedLayerForward(const void* x, const void* w_router, const float* rout
     if (rc == MOE_OK) rc = cuda_status(moe::launch_select(sel, MOE_DT_FLOAT, s));
     if (rc != MOE_OK) return rc;
     trace_mark(ev, 1, s);
-    rc = run_ffn(x, expert_ids, expert_weights, expert_out, T, H, E, K, I, workspace, L.l.f, s, ev);
+    // the permutation clears the call's error word, or sets it to what the gate recorded
+    rc = run_ffn(x, expert_ids, expert_weights, expert_out, T, H, E, K, I, workspace, L.l.f, s, ev,
+                 moe::linear_error_word());
+    up.err = down.err = at<int>(workspace, L.l.f.p.err);
     if (rc != MOE_OK) return rc;
     rc = cuda_status(moe::launch_combine(static_cast<const __half*>(expert_out), static_cast<const __half*>(weights),
                                          static_cast<__half*>(y), (int)T, (int)H, (int)K, s));
@@ -518,21 +538,9 @@ int MoeGetDeviceError(const void* workspace, int* code, void* stream)
     return MOE_OK;
 }
 
-int MoeRoutingGetDeviceError(int* code, void* stream)
-{
-    if (!code) return MOE_ERR_NULL_POINTER;
-    int* word = moe::routing_error_word();
-    if (!word) return cuda_status(cudaErrorInvalidSymbol);
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
-    int v = 0;
-    cudaError_t e = cudaMemcpyAsync(&v, word, sizeof(int), cudaMemcpyDeviceToHost, s);
-    if (e == cudaSuccess) e = cudaMemsetAsync(word, 0, sizeof(int), s);
-    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
-    if (e != cudaSuccess) return cuda_status(e);
-    *code = v;
-    return MOE_OK;
-}
+int MoeRoutingGetDeviceError(int* code, void* stream) { return take_error_word(moe::routing_error_word, code, stream); }
 
+int MoeLinearGetDeviceError(int* code, void* stream) { return take_error_word(moe::linear_error_word, code, stream); }
 const char* MoeStatusString(int status)
 {
     switch (status) {

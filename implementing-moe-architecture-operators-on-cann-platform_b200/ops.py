@@ -78,6 +78,7 @@ def lib():
         L.MoeRouterSelect.argtypes = [_vp, _int, _i64, _vp, _vp, _vp, _int] + [_i64] * 5 + [
             _int, _int, _int, ctypes.c_float, _vp]
         L.MoeLinear.argtypes = [_vp] * 5 + [_i64] * 7 + [_int] * 4 + [_vp]
+        L.MoeLinearGetDeviceError.argtypes = [_intp, _vp]
         L.MoeSharedLayerWorkspaceSize.argtypes = [_i64] * 6
         L.MoeSharedLayerWorkspaceSize.restype = _sz
         L.MoeSharedLayerForward.argtypes = [_vp] * 9 + [_i64] * 8 + [_int] * 3 + [ctypes.c_float, _vp, _sz, _vp]

@@ -272,6 +272,12 @@ int MoePermute(const int32_t* expert_ids, int32_t* perm, int32_t* expert_offsets
  * share the word.  No counterpart in the reference (its kernels return void). */
 int MoeRoutingGetDeviceError(int* code, void* stream);
 
+/* The same for MoeLinear, which has no workspace either: synchronises `stream`, writes
+ * the word its bounded waits record into (2/4/8 = a copy, tensor-core or epilogue wait
+ * gave up; never expected) to *code and clears it.  MoeSharedLayerForward moves the word
+ * into its own error word. */
+int MoeLinearGetDeviceError(int* code, void* stream);
+
 /* Synchronises `stream` and reads the device error word of a MoeExpertFFN,
  * MoeLayerForward, MoePermute or MoeEpLayerForward workspace into *code (0 = none;
  * 1 = expert id out of range; 2/4/8 = a grouped-GEMM wait timed out; expert
