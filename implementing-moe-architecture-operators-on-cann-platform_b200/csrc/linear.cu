@@ -88,23 +88,128 @@ __device__ __forceinline__ void lin_store(void* p, size_t i, float v, int type)
     else
         static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
 }
-__device__ __forceinline__ uint32_t lin_pack(float a, float b, int type)
+// The type of y, fixed at compile time where it is used per element.
+template <int OT>
+struct LinOut;
+template <>
+struct LinOut<MOE_DT_FLOAT> {
+    typedef float T;
+    static __device__ __forceinline__ float to(float v) { return v; }
+    static __device__ __forceinline__ float from(float v) { return v; }
+};
+template <>
+struct LinOut<MOE_DT_FLOAT16> {
+    typedef __half T;
+    static __device__ __forceinline__ __half to(float v) { return __float2half_rn(v); }
+    static __device__ __forceinline__ float from(__half v) { return __half2float(v); }
+    static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_half2(a, b); }
+    static __device__ __forceinline__ float2 unpack(uint32_t q) { return __half22float2(*reinterpret_cast<__half2*>(&q)); }
+};
+template <>
+struct LinOut<MOE_DT_BF16> {
+    typedef __nv_bfloat16 T;
+    static __device__ __forceinline__ __nv_bfloat16 to(float v) { return __float2bfloat16_rn(v); }
+    static __device__ __forceinline__ float from(__nv_bfloat16 v) { return __bfloat162float(v); }
+    static __device__ __forceinline__ uint32_t pack(float a, float b)
+    {
+        __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<uint32_t*>(&h);
+    }
+    static __device__ __forceinline__ float2 unpack(uint32_t q)
+    {
+        return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&q));
+    }
+};
+
+// 16 bytes of y <-> floats (8 of a 16-bit type, 4 of fp32)
+template <int OT>
+__device__ __forceinline__ uint4 lin_pack16(const float* v)
 {
-    if (type == MOE_DT_FLOAT16) return pack_half2(a, b);
-    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<uint32_t*>(&h);
+    if constexpr (OT == MOE_DT_FLOAT)
+        return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    else
+        return make_uint4(LinOut<OT>::pack(v[0], v[1]), LinOut<OT>::pack(v[2], v[3]), LinOut<OT>::pack(v[4], v[5]),
+                          LinOut<OT>::pack(v[6], v[7]));
 }
-__device__ __forceinline__ float2 lin_unpack(uint32_t q, int type)
+template <int OT>
+__device__ __forceinline__ void lin_add16(float* v, uint4 q)
 {
-    if (type == MOE_DT_FLOAT16) return __half22float2(*reinterpret_cast<const __half2*>(&q));
-    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&q));
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (OT == MOE_DT_FLOAT) {
+            v[i] += __uint_as_float(w[i]);
+        } else {
+            const float2 f = LinOut<OT>::unpack(w[i]);
+            v[2 * i] += f.x;
+            v[2 * i + 1] += f.y;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------- waits
+// Bounded wait for a phase of an mbarrier (CLUSTER: completed by the peer CTA too).  The
+// clock is read only after a first round of tries: reading %globaltimer takes longer than
+// most of these waits.
+template <bool CLUSTER>
+__device__ __forceinline__ bool lin_try(uint32_t bar, uint32_t parity)
+{
+    return CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity);
+}
+template <bool CLUSTER>
+__device__ __noinline__ bool lin_wait_slow(uint32_t bar, uint32_t parity, int* err, int code, volatile int* abort_flag)
+{
+    const uint64_t t0 = global_timer_ns();
+    for (;;) {
+        for (int i = 0; i < 64; i++)
+            if (lin_try<CLUSTER>(bar, parity)) return true;
+        if (*abort_flag) return false;
+        if (global_timer_ns() - t0 > MOE_WAIT_LIMIT_NS) {
+            atomicOr(err, code);
+            *abort_flag = 1;
+            return false;
+        }
+    }
+}
+template <bool CLUSTER>
+__device__ __forceinline__ bool lin_wait(uint32_t bar, uint32_t parity, int* err, int code, volatile int* abort_flag)
+{
+    for (int i = 0; i < 64; i++)
+        if (lin_try<CLUSTER>(bar, parity)) return true;
+    return lin_wait_slow<CLUSTER>(bar, parity, err, code, abort_flag);
+}
+
+// The same without a way out but the clock: the UMMAs in flight must be done before TMEM
+// is freed, whatever else gave up.
+template <bool CLUSTER>
+__device__ __forceinline__ void lin_drain(uint32_t bar, int* err)
+{
+    for (int i = 0; i < 64; i++)
+        if (lin_try<CLUSTER>(bar, 0)) return;
+    const uint64_t t0 = global_timer_ns();
+    while (!lin_try<CLUSTER>(bar, 0))
+        if (global_timer_ns() - t0 > MOE_WAIT_LIMIT_NS) {
+            atomicOr(err, MOE_DEV_WAIT_TIMEOUT_MMA);
+            return;
+        }
+}
+
+// One lane of a converged warp, the way that lets the compiler know it is one: with
+// lane == 0 in its place a stage's three copies took about 500 cycles to issue, and its four
+// UMMAs with their commit 600, more than the 256 or 512 cycles that the products take.
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
 }
 
 // ---------------------------------------------------------------------- tensor-core tiles
 constexpr int LG_BM = 128;                     // tokens per CTA and tile (UMMA M)
 constexpr int LG_BK = 64;                      // k per stage: one 128-byte swizzle row
 constexpr int LG_A_BYTES = LG_BM * LG_BK * 2;  // 16 KB
-constexpr int LG_THREADS = 192;
+constexpr int LG_EPI_WARPS = 8;                // two per TMEM lane quarter, taking chunks in turn
+constexpr int LG_THREADS = 64 + 32 * LG_EPI_WARPS;  // narrow tiles: one warp more
 constexpr int LG_MAX_STAGES = 8;
 constexpr int LG_GROUP_M = 8;                  // m tiles that run together over all n tiles
 
@@ -114,10 +219,18 @@ template <int PAIR, int BN>
 struct LinCfg {
     static_assert(BN == 256 || (BN == 128 && !PAIR), "tile");
     static constexpr int B_HALF = (BN / 2) * LG_BK * 2;  // bytes of one box of w
-    static constexpr int STAGE_BYTES = LG_A_BYTES + (PAIR ? B_HALF : 2 * B_HALF);
-    static constexpr int STAGES = PAIR ? 6 : (BN == 256 ? 4 : 6);
+    static constexpr int KB_BYTES = LG_A_BYTES + (PAIR ? B_HALF : 2 * B_HALF);
+    // k blocks per stage: with 128 columns the four UMMAs of one run for 256 cycles, little
+    // more than their issue, commit and wait
+    static constexpr int KPS = BN == 128 ? 2 : 1;
+    static constexpr int STAGE_BYTES = KPS * KB_BYTES;
+    static constexpr int STAGES = PAIR ? 6 : (BN == 256 ? 4 : 3);
     static constexpr int ROWS = PAIR ? 2 * LG_BM : LG_BM;
     static constexpr uint32_t TMEM_COLS = 2 * BN;
+    // A copy takes about 95 cycles to issue; a k block of a narrow tile runs 256 and needs
+    // three: x then has a warp of its own.
+    static constexpr bool X_WARP = BN == 128;
+    static constexpr int THREADS = LG_THREADS + (X_WARP ? 32 : 0);
 };
 
 struct LinTail {
@@ -126,20 +239,22 @@ struct LinTail {
     uint64_t tfull[2];
     uint64_t tempty[2];
     uint64_t drain;
+    uint64_t recv;  // (k split) the partial sums of this CTA's columns
     uint32_t tmem_base;
     int abort_flag;
 };
 constexpr size_t LG_TAIL = (sizeof(LinTail) + 127) & ~(size_t)127;
 
-// Staging of one 32-column chunk per epilogue warp: 32 rows x 32 floats, padded to 144
-// bytes so that row-wise writes and transposed reads both hit every bank once.
-constexpr int LG_STG_ROW = 144;
+// Staging for the epilogue's stores, per warp: 32 rows of 64 bytes (32 columns of a 16-bit
+// type, 16 of fp32), padded to 80 bytes so that row-wise writes and transposed reads both
+// spread over the banks.
+constexpr int LG_STG_ROW = 80;
 constexpr int LG_STG_WARP = 32 * LG_STG_ROW;
 
 template <int PAIR, int BN>
 __host__ __device__ constexpr size_t lin_smem_bytes()
 {
-    return 1024 + (size_t)LinCfg<PAIR, BN>::STAGES * LinCfg<PAIR, BN>::STAGE_BYTES + LG_TAIL + 4 * LG_STG_WARP;
+    return 1024 + (size_t)LinCfg<PAIR, BN>::STAGES * LinCfg<PAIR, BN>::STAGE_BYTES + LG_TAIL + LG_EPI_WARPS * LG_STG_WARP;
 }
 static_assert(lin_smem_bytes<1, 256>() <= 227 * 1024 && lin_smem_bytes<0, 256>() <= 227 * 1024 &&
                   lin_smem_bytes<0, 128>() <= 227 * 1024, "smem");
@@ -155,6 +270,7 @@ struct LinParams {
     int act, gated;
     int vec_y, vec_r;    // rows of y / residual start on 16-byte boundaries
     int mt, nt;          // tiles
+    int x_rows;          // tokens per box of x: 128, or fewer when T is smaller
     int w_evict_first;   // w is read by one m tile only
 };
 
@@ -165,83 +281,18 @@ __host__ __device__ constexpr uint32_t lin_idesc(int M, int N, bool bf16)
 
 // Tile index -> (m, n): LG_GROUP_M m tiles run together over all n tiles, so that a
 // group's x stays in L2 while w passes by once per group.
-__device__ __forceinline__ void lin_tile(const LinParams& p, long long tile, int& m, int& n)
+__device__ __forceinline__ void lin_tile(const LinParams& p, uint32_t tile, int& m, int& n)
 {
-    const long long width = (long long)LG_GROUP_M * p.nt;
-    const int g = (int)(tile / width);
-    const int r = (int)(tile - g * width);
-    const int gm = min(LG_GROUP_M, p.mt - g * LG_GROUP_M);
-    n = r / gm;
-    m = g * LG_GROUP_M + (r - n * gm);
-}
-
-// Writes one 32-column chunk of a warp's 32 rows: v[c] is column col0 + c of this lane's
-// row, before the residual.  Through shared memory, so that each store instruction covers
-// whole 64-byte (fp32: 128-byte) row segments.  row0: the warp's first row; rows: how many
-// of its rows exist.
-__device__ __forceinline__ void lin_store_chunk(const LinParams& p, uint8_t* stg, int lane, const float (&v)[32],
-                                                int row0, int rows, int col0)
-{
-    float4* mine = reinterpret_cast<float4*>(stg + lane * LG_STG_ROW);
-#pragma unroll
-    for (int i = 0; i < 8; i++) mine[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-    __syncwarp();
-    if (p.otype == MOE_DT_FLOAT) {
-        const int c = (lane & 7) * 4, n = col0 + c;
-#pragma unroll 4
-        for (int i = 0; i < 8; i++) {
-            const int r = 4 * i + (lane >> 3);
-            if (r >= rows || n >= p.N) continue;
-            float4 q = *reinterpret_cast<const float4*>(stg + r * LG_STG_ROW + c * 4);
-            float* dst = static_cast<float*>(p.y) + (size_t)(row0 + r) * p.ldy + n;
-            const float* res = p.residual ? static_cast<const float*>(p.residual) + (size_t)(row0 + r) * p.ldr + n : nullptr;
-            const int left = p.N - n;
-            if (left >= 4 && p.vec_y && (!res || p.vec_r)) {
-                if (res) {
-                    const float4 a = *reinterpret_cast<const float4*>(res);
-                    q = make_float4(q.x + a.x, q.y + a.y, q.z + a.z, q.w + a.w);
-                }
-                *reinterpret_cast<float4*>(dst) = q;
-            } else {
-                const float e[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (j < left) dst[j] = e[j] + (res ? res[j] : 0.0f);
-            }
-        }
-    } else {
-        const int c = (lane & 3) * 8, n = col0 + c;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int r = 8 * i + (lane >> 2);
-            if (r >= rows || n >= p.N) continue;
-            const float4 q0 = *reinterpret_cast<const float4*>(stg + r * LG_STG_ROW + c * 4);
-            const float4 q1 = *reinterpret_cast<const float4*>(stg + r * LG_STG_ROW + c * 4 + 16);
-            float e[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
-            __half* dst = static_cast<__half*>(p.y) + (size_t)(row0 + r) * p.ldy + n;
-            const __half* res = p.residual ? static_cast<const __half*>(p.residual) + (size_t)(row0 + r) * p.ldr + n : nullptr;
-            const int left = p.N - n;
-            if (left >= 8 && p.vec_y && (!res || p.vec_r)) {
-                if (res) {
-                    const uint4 a = *reinterpret_cast<const uint4*>(res);
-                    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const float2 f = lin_unpack(w[j], p.otype);
-                        e[2 * j] += f.x;
-                        e[2 * j + 1] += f.y;
-                    }
-                }
-                *reinterpret_cast<uint4*>(dst) = make_uint4(lin_pack(e[0], e[1], p.otype), lin_pack(e[2], e[3], p.otype),
-                                                            lin_pack(e[4], e[5], p.otype), lin_pack(e[6], e[7], p.otype));
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; j++)
-                    if (j < left) lin_store(dst, j, e[j] + (res ? lin_load(res, j, p.otype) : 0.0f), p.otype);
-            }
-        }
+    const uint32_t width = LG_GROUP_M * (uint32_t)p.nt;
+    uint32_t g = 0, r = tile;
+    if (tile >= width) {
+        g = tile / width;
+        r = tile - g * width;
     }
-    __syncwarp();
+    const uint32_t gm = min((uint32_t)LG_GROUP_M, (uint32_t)p.mt - g * LG_GROUP_M);
+    const uint32_t nn = gm == LG_GROUP_M ? r / LG_GROUP_M : r / gm;
+    n = (int)nn;
+    m = (int)(g * LG_GROUP_M + (r - nn * gm));
 }
 
 // v[c] += bias[col + c]: each lane fetches one column's bias, the warp shares them.
@@ -252,8 +303,117 @@ __device__ __forceinline__ void lin_add_bias(const LinParams& p, int lane, int n
     for (int c = 0; c < 32; c++) v[c] += __shfl_sync(0xffffffffu, b, c);
 }
 
+// One warp's 32 rows x `cols` outputs of a tile: accumulators from TMEM (tbase; the up
+// sums of a gated tile `up` columns further), bias, activation, gate, residual, store.
+// A chunk of 32 columns at a time (every other one: `half`), straight-line: an SM runs two
+// such warps per scheduler, so most dependent instructions are waited for.  Stores and residual loads go through
+// shared memory, so that each instruction covers whole 64-byte row segments.
+template <int OT>
+__device__ __forceinline__ void lin_epilogue(const LinParams& p, uint32_t tbase, int up, uint8_t* stg, int lane, int row0,
+                                             int rows, int col0, int cols, int half)
+{
+    typedef typename LinOut<OT>::T TO;
+    constexpr int HALVES = OT == MOE_DT_FLOAT ? 2 : 1;  // 64-byte pieces of a 32-column chunk
+    constexpr int HC = 32 / HALVES;                     // columns per piece
+    constexpr int E16 = 16 / (int)sizeof(TO);           // elements of 16 bytes
+    uint4* const mine = reinterpret_cast<uint4*>(stg + lane * LG_STG_ROW);
+    // the transposed view: lane -> rows r0 + 8 i, 16-byte piece c0 of the 64
+    const int r0 = lane >> 2, c0 = lane & 3;
+    const uint4* const trans = reinterpret_cast<const uint4*>(stg + r0 * LG_STG_ROW + c0 * 16);
+    const bool aligned = p.vec_y && (!p.residual || p.vec_r);
+    TO* const y = static_cast<TO*>(p.y) + (size_t)row0 * p.ldy + col0;
+    const TO* const res = p.residual ? static_cast<const TO*>(p.residual) + (size_t)row0 * p.ldr + col0 : nullptr;
+    const int valid = min(cols, p.N - col0);
+#pragma unroll 1
+    for (int j = 32 * half; j < valid; j += 64) {
+        uint32_t a[32];
+        float v[32];
+        tmem_ld_32x32b_x32(tbase + j, a);
+        const bool fast = aligned && j + 32 <= valid;
+        uint4 rq[HALVES * 4];
+        if (res && fast) {
+#pragma unroll
+            for (int h = 0; h < HALVES; h++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (r0 + 8 * i < rows)
+                        rq[h * 4 + i] = *reinterpret_cast<const uint4*>(res + (size_t)(r0 + 8 * i) * p.ldr + j + h * HC +
+                                                                         c0 * E16);
+        }
+        if (p.gated) {
+            uint32_t b[32];
+            float u[32];
+            tmem_ld_32x32b_x32(tbase + up + j, b);
+            tmem_ld_wait();
+#pragma unroll
+            for (int c = 0; c < 32; c++) {
+                v[c] = __uint_as_float(a[c]);
+                u[c] = __uint_as_float(b[c]);
+            }
+            if (p.bias) {
+                lin_add_bias(p, lane, col0 + j, 0, v);
+                lin_add_bias(p, lane, col0 + j, p.N, u);
+            }
+            lin_act(v, p.act);
+#pragma unroll
+            for (int c = 0; c < 32; c++) v[c] *= u[c];
+        } else {
+            tmem_ld_wait();
+#pragma unroll
+            for (int c = 0; c < 32; c++) v[c] = __uint_as_float(a[c]);
+            if (p.bias) lin_add_bias(p, lane, col0 + j, 0, v);
+            lin_act(v, p.act);
+        }
+        if (fast) {
+#pragma unroll
+            for (int h = 0; h < HALVES; h++) {
+                if (res) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        *reinterpret_cast<uint4*>(stg + (r0 + 8 * i) * LG_STG_ROW + c0 * 16) = rq[h * 4 + i];
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 4; i++) lin_add16<OT>(v + h * HC + i * E16, mine[i]);
+                    __syncwarp();
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) mine[i] = lin_pack16<OT>(v + h * HC + i * E16);
+                __syncwarp();
+                uint4 o[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[i] = trans[i * 8 * LG_STG_ROW / 16];
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (r0 + 8 * i < rows)
+                        *reinterpret_cast<uint4*>(y + (size_t)(r0 + 8 * i) * p.ldy + j + h * HC + c0 * E16) = o[i];
+                __syncwarp();
+            }
+        } else {
+            // rows off 16-byte boundaries, or the last columns: half a warp per row, an
+            // element per lane, in fp32 through the staging rows
+            const int rr = lane >> 4, c = lane & 15;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) mine[i] = lin_pack16<MOE_DT_FLOAT>(v + h * 16 + i * 4);
+                __syncwarp();
+                const int n = j + h * 16 + c;
+                if (n < valid) {
+#pragma unroll 8
+                    for (int r = rr; r < rows; r += 2) {
+                        float f = *reinterpret_cast<const float*>(stg + r * LG_STG_ROW + c * 4);
+                        if (res) f += LinOut<OT>::from(res[(size_t)r * p.ldr + n]);
+                        y[(size_t)r * p.ldy + n] = LinOut<OT>::to(f);
+                    }
+                }
+                __syncwarp();
+            }
+        }
+    }
+}
+
 template <int PAIR, int BN>
-__global__ void __launch_bounds__(LG_THREADS, 1)
+__global__ void __launch_bounds__((LinCfg<PAIR, BN>::THREADS), 1)
 linear_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
                    const LinParams p)
 {
@@ -261,12 +421,13 @@ linear_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
     constexpr int STAGES = Cfg::STAGES;
     constexpr int STAGE_BYTES = Cfg::STAGE_BYTES;
     constexpr int ROWS = Cfg::ROWS;
+    constexpr int KPS = Cfg::KPS;
     extern __shared__ uint8_t lg_smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(
         (reinterpret_cast<uintptr_t>(lg_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     LinTail* tail = reinterpret_cast<LinTail*>(smem + STAGES * STAGE_BYTES);
 
-    const int warp = threadIdx.x >> 5;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // uniform, and known to be
     const int lane = threadIdx.x & 31;
     int* err = p.err ? p.err : &g_linear_err;
     // Pair mode: rank 0 of the cluster issues the UMMAs and owns the barriers they wait on.
@@ -277,12 +438,12 @@ linear_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; s++) {
-            mbar_init(smem_u32(&tail->full[s]), 1);
+            mbar_init(smem_u32(&tail->full[s]), Cfg::X_WARP ? 2 : 1);
             mbar_init(smem_u32(&tail->empty[s]), 1);
         }
         for (int a = 0; a < 2; a++) {
             mbar_init(smem_u32(&tail->tfull[a]), 1);
-            mbar_init(smem_u32(&tail->tempty[a]), PAIR ? 8 : 4);  // one arrival per epilogue warp
+            mbar_init(smem_u32(&tail->tempty[a]), (PAIR ? 2 : 1) * LG_EPI_WARPS);  // one arrival per epilogue warp
         }
         mbar_init(smem_u32(&tail->drain), 1);
         tail->abort_flag = 0;
@@ -309,30 +470,31 @@ linear_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
     pdl_wait();  // inputs come from, and y may still be read by, the launches before
 
     const uint32_t tmem_base = tail->tmem_base;
-    const long long total = (long long)p.mt * p.nt;
+    const int total = p.mt * p.nt;  // below 2^29: the host checks
     const int nk = p.nk;
     volatile int* abort_flag = &tail->abort_flag;
 
-    if (warp == 0) {
-        // ---------------------------------------------------------------- producer
-        if (lane == 0) {
+    if (warp == 0 || (Cfg::X_WARP && warp == 2 + LG_EPI_WARPS)) {
+        // ---------------------------------------------------------------- producers
+        if (elect_one()) {
             const uint64_t pol_x = l2_policy_evict_last();
             const uint64_t pol_w = p.w_evict_first ? l2_policy_evict_first() : l2_policy_evict_last();
+            const bool do_w = warp == 0, do_x = !Cfg::X_WARP || warp != 0;
+            const uint32_t kb_tx = (do_w ? Cfg::KB_BYTES - LG_A_BYTES : 0) + (do_x ? p.x_rows * LG_BK * 2 : 0);
             uint32_t it = 0;
             bool ok = true;
-            for (long long tile = unit; ok && tile < total; tile += nunits) {
+            for (int tile = unit; ok && tile < total; tile += nunits) {
                 int m, n;
                 lin_tile(p, tile, m, n);
                 const int x_row = m * ROWS + (int)crank * LG_BM;
                 const int w_lo = n * (p.gated ? BN / 2 : BN);
                 const int w_hi = p.gated ? p.N + w_lo : w_lo + BN / 2;
-                for (int kb = 0; kb < nk; kb++, it++) {
+                for (int kb = 0; kb < nk; kb += KPS, it++) {
                     const int s = it % STAGES;
                     const uint32_t par = ((it / STAGES) & 1u) ^ 1u;
-                    const bool got = PAIR ? mbar_wait_bounded_cluster(smem_u32(&tail->empty[s]), par, err,
-                                                                      MOE_DEV_WAIT_TIMEOUT_TMA, abort_flag)
-                                          : mbar_wait_bounded(smem_u32(&tail->empty[s]), par, err,
-                                                              MOE_DEV_WAIT_TIMEOUT_TMA, abort_flag);
+                    // the first round finds every stage empty
+                    const bool got = it < (uint32_t)STAGES || lin_wait<PAIR != 0>(smem_u32(&tail->empty[s]), par, err,
+                                                                                MOE_DEV_WAIT_TIMEOUT_TMA, abort_flag);
                     if (!got) {
                         ok = false;
                         break;
@@ -343,14 +505,22 @@ linear_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
                         // both CTAs' copies complete on the leader's barrier, which
                         // expects the bytes of both
                         const uint32_t full_leader = mapa_shared(full, 0);
-                        if (leader) mbar_arrive_expect_tx(full, 2 * STAGE_BYTES);
+                        if (leader) mbar_arrive_expect_tx(full, 2 * kb_tx);
                         tma_load_2d_pair(st, &tmX, full_leader, kb * LG_BK, x_row, pol_x);
                         tma_load_2d_pair(st + LG_A_BYTES, &tmW, full_leader, kb * LG_BK, leader ? w_lo : w_hi, pol_w);
                     } else {
-                        mbar_arrive_expect_tx(full, STAGE_BYTES);
-                        tma_load_2d(st, &tmX, full, kb * LG_BK, x_row, pol_x);
-                        tma_load_2d(st + LG_A_BYTES, &tmW, full, kb * LG_BK, w_lo, pol_w);
-                        tma_load_2d(st + LG_A_BYTES + Cfg::B_HALF, &tmW, full, kb * LG_BK, w_hi, pol_w);
+                        const int nb = min(KPS, nk - kb);
+                        mbar_arrive_expect_tx(full, nb * kb_tx);
+#pragma unroll
+                        for (int i = 0; i < KPS; i++) {
+                            if (i >= nb) break;
+                            const uint32_t dst = st + i * Cfg::KB_BYTES;
+                            if (do_x) tma_load_2d(dst, &tmX, full, (kb + i) * LG_BK, x_row, pol_x);
+                            if (do_w) {
+                                tma_load_2d(dst + LG_A_BYTES, &tmW, full, (kb + i) * LG_BK, w_lo, pol_w);
+                                tma_load_2d(dst + LG_A_BYTES + Cfg::B_HALF, &tmW, full, (kb + i) * LG_BK, w_hi, pol_w);
+                            }
+                        }
                     }
                 }
             }
@@ -367,42 +537,39 @@ linear_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
         }
     } else if (warp == 1) {
         // ---------------------------------------------------------------- UMMA issuer
-        if (lane == 0 && leader) {
+        if (leader && elect_one()) {
             const uint32_t idesc = lin_idesc(ROWS, BN, p.type == MOE_DT_BF16);
             uint32_t it = 0, lt = 0;
             bool ok = true;
-            for (long long tile = unit; ok && tile < total; tile += nunits, lt++) {
+            for (int tile = unit; ok && tile < total; tile += nunits, lt++) {
                 const uint32_t acc = lt & 1u;
                 const uint32_t tpar = ((lt >> 1) & 1u) ^ 1u;
-                if (!(PAIR ? mbar_wait_bounded_cluster(smem_u32(&tail->tempty[acc]), tpar, err,
-                                                       MOE_DEV_WAIT_TIMEOUT_MMA, abort_flag)
-                           : mbar_wait_bounded(smem_u32(&tail->tempty[acc]), tpar, err, MOE_DEV_WAIT_TIMEOUT_MMA,
-                                               abort_flag)))
+                if (!(lin_wait<PAIR != 0>(smem_u32(&tail->tempty[acc]), tpar, err, MOE_DEV_WAIT_TIMEOUT_MMA, abort_flag)))
                     break;
                 tc_fence_after();
                 const uint32_t d = tmem_base + acc * BN;
-                for (int kb = 0; kb < nk; kb++, it++) {
+                for (int kb = 0; kb < nk; kb += KPS, it++) {
                     const int s = it % STAGES;
-                    const uint32_t fpar = (it / STAGES) & 1u;
-                    if (!(PAIR ? mbar_wait_bounded_cluster(smem_u32(&tail->full[s]), fpar, err,
-                                                           MOE_DEV_WAIT_TIMEOUT_MMA, abort_flag)
-                               : mbar_wait_bounded(smem_u32(&tail->full[s]), fpar, err, MOE_DEV_WAIT_TIMEOUT_MMA,
-                                                   abort_flag))) {
+                    if (!lin_wait<PAIR != 0>(smem_u32(&tail->full[s]), (it / STAGES) & 1u, err,
+                                                       MOE_DEV_WAIT_TIMEOUT_MMA, abort_flag)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t a_addr = smem_u32(smem + s * STAGE_BYTES);
-                    const uint32_t b_addr = a_addr + LG_A_BYTES;
 #pragma unroll
-                    for (int k = 0; k < LG_BK / 16; k++) {
-                        // k advances by 16 elements = 32 bytes inside the swizzle row
-                        if (PAIR)
-                            umma_f16_ss_pair(d, umma_desc_sw128(a_addr + k * 32), umma_desc_sw128(b_addr + k * 32),
-                                             idesc, (kb | k) != 0);
-                        else
-                            umma_f16_ss(d, umma_desc_sw128(a_addr + k * 32), umma_desc_sw128(b_addr + k * 32), idesc,
-                                        (kb | k) != 0);
+                    for (int i = 0; i < KPS; i++) {
+                        if (kb + i >= nk) break;
+                        const uint32_t a_addr = smem_u32(smem + s * STAGE_BYTES + i * Cfg::KB_BYTES);
+                        const uint32_t b_addr = a_addr + LG_A_BYTES;
+#pragma unroll
+                        for (int k = 0; k < LG_BK / 16; k++) {
+                            // k advances by 16 elements = 32 bytes inside the swizzle row
+                            const uint64_t da = umma_desc_sw128(a_addr + k * 32), db = umma_desc_sw128(b_addr + k * 32);
+                            if (PAIR)
+                                umma_f16_ss_pair(d, da, db, idesc, (kb | i | k) != 0);
+                            else
+                                umma_f16_ss(d, da, db, idesc, (kb | i | k) != 0);
+                        }
                     }
                     if (PAIR) {
                         umma_commit_pair(smem_u32(&tail->empty[s]));
@@ -425,68 +592,35 @@ linear_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
                 umma_commit_pair(smem_u32(&tail->drain));
             else
                 umma_commit(smem_u32(&tail->drain));
-            const uint64_t t0 = global_timer_ns();
-            while (!(PAIR ? mbar_try_wait_cluster(smem_u32(&tail->drain), 0) : mbar_try_wait(smem_u32(&tail->drain), 0)))
-                if (global_timer_ns() - t0 > MOE_WAIT_LIMIT_NS) {
-                    atomicOr(err, MOE_DEV_WAIT_TIMEOUT_MMA);
-                    break;
-                }
+            lin_drain<PAIR != 0>(smem_u32(&tail->drain), err);
         }
     } else {
         // ---------------------------------------------------------------- epilogue
         const int q = warp & 3;  // the TMEM lane quarter this warp may read
-        uint8_t* stg = smem + STAGES * STAGE_BYTES + LG_TAIL + (size_t)q * LG_STG_WARP;
+        uint8_t* stg = smem + STAGES * STAGE_BYTES + LG_TAIL + (size_t)(warp - 2) * LG_STG_WARP;
+        const int half = (warp - 2) >> 2;
         // in pair mode the epilogue warps of both CTAs release the leader's accumulator
         const uint32_t tempty0 = PAIR ? mapa_shared(smem_u32(&tail->tempty[0]), 0) : smem_u32(&tail->tempty[0]);
         uint32_t lt = 0;
-        for (long long tile = unit; tile < total; tile += nunits, lt++) {
+        for (int tile = unit; tile < total; tile += nunits, lt++) {
             int m, n;
             lin_tile(p, tile, m, n);
             const uint32_t acc = lt & 1u;
             const uint32_t tpar = (lt >> 1) & 1u;
-            if (!(PAIR ? mbar_wait_bounded_cluster(smem_u32(&tail->tfull[acc]), tpar, err, MOE_DEV_WAIT_TIMEOUT_EPI,
-                                                   abort_flag)
-                       : mbar_wait_bounded(smem_u32(&tail->tfull[acc]), tpar, err, MOE_DEV_WAIT_TIMEOUT_EPI,
-                                           abort_flag)))
+            if (!(lin_wait<PAIR != 0>(smem_u32(&tail->tfull[acc]), tpar, err, MOE_DEV_WAIT_TIMEOUT_EPI, abort_flag)))
                 break;
             tc_fence_after();
             const int row0 = m * ROWS + (int)crank * LG_BM + q * 32;
             const int rows = min(32, p.T - row0);  // <= 0: none of this warp's rows exist
             const uint32_t tbase = tmem_base + acc * BN + ((uint32_t)(q * 32) << 16);
             const int cols = p.gated ? BN / 2 : BN;
-            const int col0 = n * cols;
             if (rows > 0) {
-#pragma unroll 1
-                for (int j = 0; j < cols && col0 + j < p.N; j += 32) {
-                    uint32_t a[32];
-                    float v[32];
-                    tmem_ld_32x32b_x32(tbase + j, a);
-                    if (p.gated) {
-                        uint32_t b[32];
-                        float u[32];
-                        tmem_ld_32x32b_x32(tbase + BN / 2 + j, b);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int c = 0; c < 32; c++) {
-                            v[c] = __uint_as_float(a[c]);
-                            u[c] = __uint_as_float(b[c]);
-                        }
-                        if (p.bias) {
-                            lin_add_bias(p, lane, col0 + j, 0, v);
-                            lin_add_bias(p, lane, col0 + j, p.N, u);
-                        }
-                        lin_act(v, p.act);
-#pragma unroll
-                        for (int c = 0; c < 32; c++) v[c] *= u[c];
-                    } else {
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int c = 0; c < 32; c++) v[c] = __uint_as_float(a[c]);
-                        if (p.bias) lin_add_bias(p, lane, col0 + j, 0, v);
-                        lin_act(v, p.act);
-                    }
-                    lin_store_chunk(p, stg, lane, v, row0, rows, col0 + j);
-                }
+                if (p.otype == MOE_DT_FLOAT16)
+                    lin_epilogue<MOE_DT_FLOAT16>(p, tbase, BN / 2, stg, lane, row0, rows, n * cols, cols, half);
+                else if (p.otype == MOE_DT_BF16)
+                    lin_epilogue<MOE_DT_BF16>(p, tbase, BN / 2, stg, lane, row0, rows, n * cols, cols, half);
+                else
+                    lin_epilogue<MOE_DT_FLOAT>(p, tbase, BN / 2, stg, lane, row0, rows, n * cols, cols, half);
             }
             tc_fence_before();
             __syncwarp();
@@ -517,46 +651,139 @@ linear_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
 }
 
 // ---------------------------------------------------------------------- k split over a cluster
-// One 128 x 128 tile per cluster of S CTAs (S = 1, 2, 4, 8).  CTA r multiplies k blocks
-// [nk r / S, nk (r + 1) / S), then sends the columns that CTA d finishes to d's receive
-// buffer [S][128][W + 4], W = 128 / S (gated: W/2 gate and W/2 up columns), and finishes
-// its own columns from the S partial sums in rank order.
-constexpr int LS_BN = 128;
-constexpr int LS_STAGES = 4;
-constexpr int LS_STAGE_BYTES = LG_A_BYTES + LS_BN * LG_BK * 2;  // 32 KB
-constexpr int LS_MAX_S = 8;
-constexpr int LS_RECV_BYTES = LS_MAX_S * LG_BM * (LS_BN / LS_MAX_S + 4) * 4;  // the largest: 80 KB
-constexpr size_t LS_SMEM = 1024 + (size_t)LS_STAGES * LS_STAGE_BYTES + LS_RECV_BYTES + LG_TAIL;
-static_assert(LS_SMEM <= 227 * 1024, "smem");
+// One 128 x BN tile per cluster of S CTAs.  CTA r multiplies k blocks [nk r / S,
+// nk (r + 1) / S), lays its sums out as S blocks [128][W + 4], W = BN / S (gated: W/2 gate
+// and W/2 up columns), in the shared memory that its operands no longer need, and sends
+// block d to CTA d by bulk copies: stores to distributed shared memory, 16 bytes per lane,
+// took 5 us for the 64 KB where these take less than 1.  Each CTA finishes its own columns
+// from the S partial sums in rank order.
+constexpr int LS_KPS = 2;        // k blocks per stage, as in the narrow tiles
+constexpr int LS_THREADS = 256;  // w copies, UMMA, 4 TMEM readers, x copies, 1 more to finish columns
 
-__device__ __forceinline__ void st_cluster_v4(uint32_t addr, float a, float b, float c, float d)
+template <int S, int BN>
+struct SplitCfg {
+    static constexpr int W = BN / S;
+    static constexpr int PITCH = W + 4;
+    static constexpr int B_HALF = BN / 2 * LG_BK * 2;
+    static constexpr int KB_BYTES = LG_A_BYTES + 2 * B_HALF;
+    static constexpr int STAGE_BYTES = LS_KPS * KB_BYTES;
+    static constexpr int RECV_BYTES = S * LG_BM * PITCH * 4;
+    static constexpr int STAGES = BN == 64 ? 3 : 2;  // 128 or 144 KB
+    static constexpr size_t SMEM = 1024 + (size_t)STAGES * STAGE_BYTES + RECV_BYTES + LG_TAIL;
+    static_assert(W >= 16, "a gated CTA finishes at least 8 outputs");
+    static_assert(STAGES * STAGE_BYTES >= RECV_BYTES, "the sums fit the ring");
+    static_assert(SMEM <= 227 * 1024, "smem");
+};
+
+// Copies `bytes` of this CTA's shared memory to another CTA's (shared::cluster addresses),
+// counted on that CTA's mbarrier.
+__device__ __forceinline__ void copy_to_cta(uint32_t dst_cluster, uint32_t src, uint32_t bytes, uint32_t bar_cluster)
 {
-    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d)
+    asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst_cluster),
+                 "r"(src), "r"(bytes), "r"(bar_cluster)
                  : "memory");
 }
 
-__global__ void __launch_bounds__(LG_THREADS, 1)
-linear_split_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
-                    const LinParams p, const int S)
+// Finishes this CTA's columns: 8 outputs per thread and step.
+template <int S, int BN, bool GATED, int OT>
+__device__ __forceinline__ void split_finish(const LinParams& p, const float* recv, int m, int col0)
 {
+    constexpr int OUTS = GATED ? SplitCfg<S, BN>::W / 2 : SplitCfg<S, BN>::W;
+    constexpr int V = 8;
+    constexpr int GROUPS = OUTS / V;
+    constexpr int PITCH = SplitCfg<S, BN>::PITCH;
+    const int rows = min(LG_BM, p.T - m * LG_BM);
+#pragma unroll 1
+    for (int i = threadIdx.x; i < rows * GROUPS; i += LS_THREADS) {
+        const int row = i / GROUPS, g = i % GROUPS;
+        const int n = col0 + V * g, left = p.N - n;
+        if (left <= 0) continue;
+        const float* src = recv + row * PITCH + V * g;
+        float v[V] = {}, u[V] = {};
+#pragma unroll
+        for (int s = 0; s < S; s++)
+#pragma unroll
+            for (int j = 0; j < V; j += 4) {
+                const float4 a = *reinterpret_cast<const float4*>(src + s * LG_BM * PITCH + j);
+                v[j] += a.x;
+                v[j + 1] += a.y;
+                v[j + 2] += a.z;
+                v[j + 3] += a.w;
+                if (GATED) {
+                    const float4 b = *reinterpret_cast<const float4*>(src + s * LG_BM * PITCH + OUTS + j);
+                    u[j] += b.x;
+                    u[j + 1] += b.y;
+                    u[j + 2] += b.z;
+                    u[j + 3] += b.w;
+                }
+            }
+        if (p.bias) {
+#pragma unroll
+            for (int j = 0; j < V; j++)
+                if (j < left) {
+                    v[j] += lin_load(p.bias, n + j, p.type);
+                    if (GATED) u[j] += lin_load(p.bias, (size_t)p.N + n + j, p.type);
+                }
+        }
+        lin_act(v, p.act);
+        if (GATED) {
+#pragma unroll
+            for (int j = 0; j < V; j++) v[j] *= u[j];
+        }
+        typedef typename LinOut<OT>::T TO;
+        constexpr int E16 = 16 / (int)sizeof(TO);
+        const size_t t = (size_t)m * LG_BM + row;
+        TO* dst = static_cast<TO*>(p.y) + t * p.ldy + n;
+        const TO* res = p.residual ? static_cast<const TO*>(p.residual) + t * p.ldr + n : nullptr;
+        if (V % E16 == 0 && left >= V && p.vec_y && (!res || p.vec_r)) {
+#pragma unroll
+            for (int j = 0; j < V; j += E16) {
+                if (res) lin_add16<OT>(v + j, *reinterpret_cast<const uint4*>(res + j));
+                *reinterpret_cast<uint4*>(dst + j) = lin_pack16<OT>(v + j);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; j++)
+                if (j < left) dst[j] = LinOut<OT>::to(v[j] + (res ? LinOut<OT>::from(res[j]) : 0.0f));
+        }
+    }
+}
+
+template <int S, int BN, int OT>
+__device__ __forceinline__ void split_finish_any(const LinParams& p, const float* recv, int m, int col0)
+{
+    if (p.gated)
+        split_finish<S, BN, true, OT>(p, recv, m, col0);
+    else
+        split_finish<S, BN, false, OT>(p, recv, m, col0);
+}
+
+template <int S, int BN>
+__global__ void __launch_bounds__(LS_THREADS, 1)
+linear_split_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const LinParams p)
+{
+    using Cfg = SplitCfg<S, BN>;
+    constexpr int W = Cfg::W;
+    constexpr int PITCH = Cfg::PITCH;
     extern __shared__ uint8_t ls_smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(
         (reinterpret_cast<uintptr_t>(ls_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    float* recv = reinterpret_cast<float*>(smem + LS_STAGES * LS_STAGE_BYTES);
-    LinTail* tail = reinterpret_cast<LinTail*>(smem + LS_STAGES * LS_STAGE_BYTES + LS_RECV_BYTES);
+    float* recv = reinterpret_cast<float*>(smem + Cfg::STAGES * Cfg::STAGE_BYTES);
+    LinTail* tail = reinterpret_cast<LinTail*>(smem + Cfg::STAGES * Cfg::STAGE_BYTES + Cfg::RECV_BYTES);
 
-    const int warp = threadIdx.x >> 5;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // uniform, and known to be
     const int lane = threadIdx.x & 31;
     int* err = p.err ? p.err : &g_linear_err;
     const int rank = (int)cluster_ctarank();
     const int tile = (int)(blockIdx.x / S);
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < LS_STAGES; s++) {
-            mbar_init(smem_u32(&tail->full[s]), 1);
+        for (int s = 0; s < Cfg::STAGES; s++) {
+            mbar_init(smem_u32(&tail->full[s]), 2);  // the copies of w, the copies of x
             mbar_init(smem_u32(&tail->empty[s]), 1);
         }
         mbar_init(smem_u32(&tail->drain), 1);
+        mbar_init(smem_u32(&tail->recv), 1);
         tail->abort_flag = 0;
         fence_barrier_init();
         tma_prefetch_desc(&tmX);
@@ -564,9 +791,15 @@ linear_split_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
     }
     pdl_trigger();
     if (warp == 1) {
-        tmem_alloc(smem_u32(&tail->tmem_base), LS_BN);
+        tmem_alloc(smem_u32(&tail->tmem_base), BN);
         tmem_relinquish();
     }
+    int m, n;
+    lin_tile(p, tile, m, n);
+    // S slabs of 32 rows come for each of the tile's row quarters that exist
+    constexpr uint32_t SLAB = 32 * PITCH * 4;
+    const int quarters = min(4, (p.T - m * LG_BM + 31) / 32);
+    if (threadIdx.x == 0) mbar_arrive_expect_tx(smem_u32(&tail->recv), S * quarters * SLAB);
     tc_fence_before();
     cluster_sync_all();  // barriers are initialised, and every CTA's shared memory is live
     tc_fence_after();
@@ -574,166 +807,134 @@ linear_split_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
 
     const uint32_t tmem_base = tail->tmem_base;
     volatile int* abort_flag = &tail->abort_flag;
-    int m, n;
-    lin_tile(p, tile, m, n);
     const int kb0 = (int)((long long)p.nk * rank / S), kb1 = (int)((long long)p.nk * (rank + 1) / S);
-    const int cols = p.gated ? LS_BN / 2 : LS_BN;
-    const int W = LS_BN / S;       // columns a CTA finishes (gated: half of them outputs)
-    const int pitch = W + 4;
+    const int cols = p.gated ? BN / 2 : BN;
 
-    if (warp == 0) {
-        if (lane == 0) {
-            const uint64_t pol_x = l2_policy_evict_last();
-            const uint64_t pol_w = p.w_evict_first ? l2_policy_evict_first() : l2_policy_evict_last();
+    if (warp == 0 || warp == 6) {
+        // A copy takes about 95 cycles to issue, more than a third of the products it
+        // feeds: w (two boxes per k block) and x have a warp each.
+        if (elect_one()) {
+            const bool is_w = warp == 0;
+            const uint64_t pol = is_w && p.w_evict_first ? l2_policy_evict_first() : l2_policy_evict_last();
+            const uint32_t kb_tx = is_w ? 2 * Cfg::B_HALF : p.x_rows * LG_BK * 2;
             const int w_lo = n * cols;
-            const int w_hi = p.gated ? p.N + w_lo : w_lo + LS_BN / 2;
+            const int w_hi = p.gated ? p.N + w_lo : w_lo + BN / 2;
             uint32_t it = 0;
             bool ok = true;
-            for (int kb = kb0; kb < kb1; kb++, it++) {
-                const int s = it % LS_STAGES;
-                if (!mbar_wait_bounded(smem_u32(&tail->empty[s]), ((it / LS_STAGES) & 1u) ^ 1u, err,
-                                       MOE_DEV_WAIT_TIMEOUT_TMA, abort_flag)) {
+            for (int kb = kb0; kb < kb1; kb += LS_KPS, it++) {
+                const int s = it % Cfg::STAGES;
+                if (it >= (uint32_t)Cfg::STAGES && !lin_wait<false>(smem_u32(&tail->empty[s]), ((it / Cfg::STAGES) & 1u) ^ 1u,
+                                                                  err, MOE_DEV_WAIT_TIMEOUT_TMA, abort_flag)) {
                     ok = false;
                     break;
                 }
                 const uint32_t full = smem_u32(&tail->full[s]);
-                const uint32_t st = smem_u32(smem + s * LS_STAGE_BYTES);
-                mbar_arrive_expect_tx(full, LS_STAGE_BYTES);
-                tma_load_2d(st + LG_A_BYTES, &tmW, full, kb * LG_BK, w_lo, pol_w);
-                tma_load_2d(st + LG_A_BYTES + LS_BN / 2 * LG_BK * 2, &tmW, full, kb * LG_BK, w_hi, pol_w);
-                tma_load_2d(st, &tmX, full, kb * LG_BK, m * LG_BM, pol_x);
+                const uint32_t st = smem_u32(smem + s * Cfg::STAGE_BYTES);
+                const int nb = min(LS_KPS, kb1 - kb);
+                mbar_arrive_expect_tx(full, nb * kb_tx);
+#pragma unroll
+                for (int i = 0; i < LS_KPS; i++) {
+                    if (i >= nb) break;
+                    const uint32_t dst = st + i * Cfg::KB_BYTES;
+                    if (is_w) {
+                        tma_load_2d(dst + LG_A_BYTES, &tmW, full, (kb + i) * LG_BK, w_lo, pol);
+                        tma_load_2d(dst + LG_A_BYTES + Cfg::B_HALF, &tmW, full, (kb + i) * LG_BK, w_hi, pol);
+                    } else {
+                        tma_load_2d(dst, &tmX, full, (kb + i) * LG_BK, m * LG_BM, pol);
+                    }
+                }
             }
             if (!ok) {
-                const uint32_t first = it > (uint32_t)LS_STAGES ? it - LS_STAGES : 0;
+                // giving up: the copies in flight land (bounded wait) before the CTA exits
+                const uint32_t first = it > (uint32_t)Cfg::STAGES ? it - Cfg::STAGES : 0;
                 for (uint32_t j = first; j < it; j++) {
                     const uint64_t t0 = global_timer_ns();
-                    while (!mbar_try_wait(smem_u32(&tail->full[j % LS_STAGES]), (j / LS_STAGES) & 1u))
+                    while (!mbar_try_wait(smem_u32(&tail->full[j % Cfg::STAGES]), (j / Cfg::STAGES) & 1u))
                         if (global_timer_ns() - t0 > MOE_WAIT_LIMIT_NS) break;
                 }
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t idesc = lin_idesc(LG_BM, LS_BN, p.type == MOE_DT_BF16);
+        if (elect_one()) {
+            const uint32_t idesc = lin_idesc(LG_BM, BN, p.type == MOE_DT_BF16);
             uint32_t it = 0;
-            for (int kb = kb0; kb < kb1; kb++, it++) {
-                const int s = it % LS_STAGES;
-                if (!mbar_wait_bounded(smem_u32(&tail->full[s]), (it / LS_STAGES) & 1u, err, MOE_DEV_WAIT_TIMEOUT_MMA,
-                                       abort_flag))
+            for (int kb = kb0; kb < kb1; kb += LS_KPS, it++) {
+                const int s = it % Cfg::STAGES;
+                if (!lin_wait<false>(smem_u32(&tail->full[s]), (it / Cfg::STAGES) & 1u, err,
+                                               MOE_DEV_WAIT_TIMEOUT_MMA, abort_flag))
                     break;
                 tc_fence_after();
-                const uint32_t a_addr = smem_u32(smem + s * LS_STAGE_BYTES);
-                const uint32_t b_addr = a_addr + LG_A_BYTES;
 #pragma unroll
-                for (int k = 0; k < LG_BK / 16; k++)
-                    umma_f16_ss(tmem_base, umma_desc_sw128(a_addr + k * 32), umma_desc_sw128(b_addr + k * 32), idesc,
-                                (kb > kb0 || k > 0) ? 1u : 0u);
+                for (int i = 0; i < LS_KPS; i++) {
+                    if (kb + i >= kb1) break;
+                    const uint32_t a_addr = smem_u32(smem + s * Cfg::STAGE_BYTES + i * Cfg::KB_BYTES);
+                    const uint32_t b_addr = a_addr + LG_A_BYTES;
+#pragma unroll
+                    for (int k = 0; k < LG_BK / 16; k++)
+                        umma_f16_ss(tmem_base, umma_desc_sw128(a_addr + k * 32), umma_desc_sw128(b_addr + k * 32), idesc,
+                                    (kb > kb0 || i > 0 || k > 0) ? 1u : 0u);
+                }
                 umma_commit(smem_u32(&tail->empty[s]));
             }
             umma_commit(smem_u32(&tail->drain));  // all sums of this CTA are in TMEM
-            const uint64_t t0 = global_timer_ns();
-            while (!mbar_try_wait(smem_u32(&tail->drain), 0))
-                if (global_timer_ns() - t0 > MOE_WAIT_LIMIT_NS) {
-                    atomicOr(err, MOE_DEV_WAIT_TIMEOUT_MMA);
-                    break;
-                }
+            lin_drain<false>(smem_u32(&tail->drain), err);
         }
-    } else {
+    } else if (warp < 6) {
         const int q = warp & 3;
-        const int row = q * 32 + lane;
-        if (mbar_wait_bounded(smem_u32(&tail->drain), 0, err, MOE_DEV_WAIT_TIMEOUT_EPI, abort_flag)) {
+        if (q < quarters && lin_wait<false>(smem_u32(&tail->drain), 0, err, MOE_DEV_WAIT_TIMEOUT_EPI, abort_flag)) {
             tc_fence_after();
-            if (m * LG_BM + q * 32 < p.T) {
-                const uint32_t mine = smem_u32(recv) + (uint32_t)((rank * LG_BM + row) * pitch) * 4u;
-#pragma unroll 1
-                for (int j = 0; j < LS_BN; j += 32) {
-                    uint32_t a[32];
-                    tmem_ld_32x32b_x32(tmem_base + ((uint32_t)(q * 32) << 16) + j, a);
-                    tmem_ld_wait();
+            // block d's row of this lane: the ring's operands have been consumed
+            float* const mine = reinterpret_cast<float*>(smem) + (q * 32 + lane) * PITCH;
 #pragma unroll
-                    for (int c = 0; c < 32; c += 4) {
-                        const int col = j + c;
-                        int d, off;
-                        if (p.gated) {
-                            const int half = col >> 6, cc = col & 63, hw = W >> 1;
-                            d = cc / hw;
-                            off = half * hw + (cc - d * hw);
-                        } else {
-                            d = col / W;
-                            off = col - d * W;
-                        }
-                        st_cluster_v4(mapa_shared(mine + (uint32_t)off * 4u, (uint32_t)d), __uint_as_float(a[c]),
-                                      __uint_as_float(a[c + 1]), __uint_as_float(a[c + 2]), __uint_as_float(a[c + 3]));
-                    }
+            for (int j = 0; j < BN; j += 32) {
+                uint32_t a[32];
+                tmem_ld_32x32b_x32(tmem_base + ((uint32_t)(q * 32) << 16) + j, a);
+                tmem_ld_wait();
+#pragma unroll
+                for (int c = 0; c < 32; c += 4) {
+                    const int col = j + c;
+                    // gated: the first BN / 2 columns are gate sums, the others up sums
+                    const int d = p.gated ? col % (BN / 2) / (W / 2) : col / W;
+                    const int off = p.gated ? col / (BN / 2) * (W / 2) + col % (BN / 2) % (W / 2) : col % W;
+                    *reinterpret_cast<float4*>(mine + d * LG_BM * PITCH + off) =
+                        make_float4(__uint_as_float(a[c]), __uint_as_float(a[c + 1]), __uint_as_float(a[c + 2]),
+                                    __uint_as_float(a[c + 3]));
                 }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane < S) {
+                const uint32_t src = smem_u32(smem) + (uint32_t)((lane * LG_BM + q * 32) * PITCH) * 4u;
+                const uint32_t dst = smem_u32(recv) + (uint32_t)((rank * LG_BM + q * 32) * PITCH) * 4u;
+                copy_to_cta(mapa_shared(dst, (uint32_t)lane), src, SLAB, mapa_shared(smem_u32(&tail->recv), (uint32_t)lane));
             }
         }
         tc_fence_before();
     }
     __syncwarp();
-    cluster_sync_all();  // every partial sum has arrived
+    // Every partial sum of this CTA's columns has arrived (or a wait gave up).  One thread
+    // looks: 256 that poll slow down what they wait for.
+    if (threadIdx.x == 0) lin_wait<true>(smem_u32(&tail->recv), 0, err, MOE_DEV_WAIT_TIMEOUT_EPI, abort_flag);
+    __syncthreads();
+    const bool arrived = *abort_flag == 0;
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem_base, LS_BN);
+        tmem_dealloc(tmem_base, BN);
     }
-
-    // this CTA's columns: 4 outputs per thread and step
-    const int outs = p.gated ? W / 2 : W;
-    const int groups = outs / 4;
-    const int col0 = n * cols + rank * outs;
-    for (int i = threadIdx.x; i < LG_BM * groups; i += LG_THREADS) {
-        const int row = i / groups, g = i - row * groups;
-        const int t = m * LG_BM + row, nn = col0 + 4 * g;
-        if (t >= p.T) break;
-        if (nn >= p.N) continue;
-        float v[4] = {}, u[4] = {};
-        for (int s = 0; s < S; s++) {
-            const float* src = recv + (size_t)(s * LG_BM + row) * pitch + 4 * g;
-            const float4 a = *reinterpret_cast<const float4*>(src);
-            v[0] += a.x;
-            v[1] += a.y;
-            v[2] += a.z;
-            v[3] += a.w;
-            if (p.gated) {
-                const float4 b = *reinterpret_cast<const float4*>(src + outs);
-                u[0] += b.x;
-                u[1] += b.y;
-                u[2] += b.z;
-                u[3] += b.w;
-            }
-        }
-        const int left = p.N - nn;
-        if (p.bias) {
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (j < left) {
-                    v[j] += lin_load(p.bias, nn + j, p.type);
-                    if (p.gated) u[j] += lin_load(p.bias, (size_t)p.N + nn + j, p.type);
-                }
-        }
-        lin_act(v, p.act);
-        if (p.gated) {
-#pragma unroll
-            for (int j = 0; j < 4; j++) v[j] *= u[j];
-        }
-        if (p.residual) {
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (j < left) v[j] += lin_load(p.residual, (size_t)t * p.ldr + nn + j, p.otype);
-        }
-        const size_t o = (size_t)t * p.ldy + nn;
-        if (left >= 4 && p.vec_y) {
-            if (p.otype == MOE_DT_FLOAT)
-                *reinterpret_cast<float4*>(static_cast<float*>(p.y) + o) = make_float4(v[0], v[1], v[2], v[3]);
-            else
-                *reinterpret_cast<uint2*>(static_cast<__half*>(p.y) + o) =
-                    make_uint2(lin_pack(v[0], v[1], p.otype), lin_pack(v[2], v[3], p.otype));
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (j < left) lin_store(p.y, o + j, v[j], p.otype);
-        }
+    // no CTA leaves while its sums may still be read: all have arrived here once all have
+    // received
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    const int col0 = n * cols + rank * (cols / S);
+    if (arrived) {
+        if (p.otype == MOE_DT_FLOAT16)
+            split_finish_any<S, BN, MOE_DT_FLOAT16>(p, recv, m, col0);
+        else if (p.otype == MOE_DT_BF16)
+            split_finish_any<S, BN, MOE_DT_BF16>(p, recv, m, col0);
+        else
+            split_finish_any<S, BN, MOE_DT_FLOAT>(p, recv, m, col0);
     }
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // ---------------------------------------------------------------------- a few tokens
@@ -743,9 +944,6 @@ linear_split_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
 // memory: a product does not depend on the order of k, so lane (g, t) takes 8 consecutive
 // elements (16 bytes) of rows g and g + 8 at k = 32 c + 8 t, and of token g, and feeds
 // them to two m16n8k16 products as if they were the columns those expect.
-constexpr int LF_WARPS = 16;
-constexpr int LF_U = 2;  // k chunks of 32 per step; the next step's loads are in flight under this one's products
-
 __device__ __forceinline__ uint4 ld_stream16(const void* p)
 {
     uint4 v;
@@ -774,10 +972,15 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <bool BF16, int MT, int NT>
-__global__ void __launch_bounds__(LF_WARPS * 32, 1) linear_few_kernel(const LinearArgs a)
+// k chunks of 32 in flight per warp: 160 to 256 bytes of w per lane
+template <int MT, int NT>
+constexpr int lin_few_depth() { return MT == 2 ? (NT == 2 ? 3 : 4) : (NT == 2 ? 5 : 8); }
+
+template <bool BF16, int MT, int NT, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) linear_few_kernel(const LinearArgs a)
 {
-    __shared__ float red[LF_WARPS][NT * 8][MT * 16 + 1];
+    constexpr int D = lin_few_depth<MT, NT>();
+    __shared__ float red[WARPS][NT * 8][MT * 16 + 1];
     pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
@@ -801,48 +1004,38 @@ __global__ void __launch_bounds__(LF_WARPS * 32, 1) linear_few_kernel(const Line
         xin[j] = g + 8 * j < a.T;
         xr[j] = x + (size_t)(xin[j] ? g + 8 * j : 0) * a.ldx + 8 * t;
     }
+    // A ring of D chunks in registers: chunk c of this warp is k = chunk_k(c), two chunks
+    // (128 bytes of a row) to a warp in turn.  A slot is loaded again as soon as its chunk
+    // has been multiplied, so D - 1 chunks are always on their way.
     float acc[MT][NT][4] = {};
-    uint4 wa[LF_U][MT][2], xb[LF_U][NT];
+    uint4 wa[D][MT][2], xb[D][NT];
     const uint4 zero = make_uint4(0, 0, 0, 0);
-    constexpr int STEP = 32 * LF_U;
-    auto load = [&](int k) {
+    auto chunk_k = [&](int c) { return ((c >> 1) * WARPS + warp) * 64 + (c & 1) * 32; };
+    auto load = [&](int slot, int kk) {
+        const bool in = kk + 8 * t < a.K;
 #pragma unroll
-        for (int c = 0; c < LF_U; c++) {
-            const int kk = k + 32 * c;
-            const bool in = kk + 8 * t < a.K;
+        for (int i = 0; i < MT; i++)
 #pragma unroll
-            for (int i = 0; i < MT; i++)
+            for (int h = 0; h < 2; h++) wa[slot][i][h] = in ? ld_stream16(wr[i][h] + kk) : zero;
 #pragma unroll
-                for (int h = 0; h < 2; h++) wa[c][i][h] = in ? ld_stream16(wr[i][h] + kk) : zero;
-#pragma unroll
-            for (int j = 0; j < NT; j++)
-                xb[c][j] = (in && xin[j]) ? ld_cached16(xr[j] + kk) : zero;
-        }
+        for (int j = 0; j < NT; j++) xb[slot][j] = (in && xin[j]) ? ld_cached16(xr[j] + kk) : zero;
     };
     pdl_wait();
-    int k = warp * STEP;
-    if (k < a.K) load(k);
-    while (k < a.K) {
-        uint4 wc[LF_U][MT][2], xc[LF_U][NT];
 #pragma unroll
-        for (int c = 0; c < LF_U; c++) {
+    for (int d = 0; d < D; d++) load(d, chunk_k(d));
+    for (int c = 0; chunk_k(c) < a.K; c += D) {
 #pragma unroll
-            for (int i = 0; i < MT; i++) wc[c][i][0] = wa[c][i][0], wc[c][i][1] = wa[c][i][1];
-#pragma unroll
-            for (int j = 0; j < NT; j++) xc[c][j] = xb[c][j];
-        }
-        k += STEP * LF_WARPS;
-        if (k < a.K) load(k);
-#pragma unroll
-        for (int c = 0; c < LF_U; c++)
+        for (int d = 0; d < D; d++) {
 #pragma unroll
             for (int i = 0; i < MT; i++)
 #pragma unroll
                 for (int j = 0; j < NT; j++) {
-                    const uint4 lo = wc[c][i][0], hi = wc[c][i][1], b = xc[c][j];
+                    const uint4 lo = wa[d][i][0], hi = wa[d][i][1], b = xb[d][j];
                     mma_16816<BF16>(acc[i][j], lo.x, hi.x, lo.y, hi.y, b.x, b.y);
                     mma_16816<BF16>(acc[i][j], lo.z, hi.z, lo.w, hi.w, b.z, b.w);
                 }
+            load(d, chunk_k(c + d + D));
+        }
     }
 #pragma unroll
     for (int i = 0; i < MT; i++)
@@ -855,13 +1048,16 @@ __global__ void __launch_bounds__(LF_WARPS * 32, 1) linear_few_kernel(const Line
         }
     __syncthreads();
     const int outs = a.gated ? 16 : 16 * MT;
-    for (int i = threadIdx.x; i < outs * a.T; i += LF_WARPS * 32) {
+    for (int i = threadIdx.x; i < outs * a.T; i += WARPS * 32) {
         const int tok = i / outs, r = i - tok * outs, n = n0 + r;
         if (n >= a.N) continue;
         float v[1] = {0.0f}, u = 0.0f;
-        for (int s = 0; s < LF_WARPS; s++) v[0] += red[s][tok][r];
-        if (MT == 2 && a.gated)
-            for (int s = 0; s < LF_WARPS; s++) u += red[s][tok][16 * (MT - 1) + r];
+#pragma unroll
+        for (int s = 0; s < WARPS; s++) v[0] += red[s][tok][r];
+        if (MT == 2 && a.gated) {
+#pragma unroll
+            for (int s = 0; s < WARPS; s++) u += red[s][tok][16 * (MT - 1) + r];
+        }
         if (a.bias) {
             v[0] += lin_load(a.bias, n, a.type);
             if (a.gated) u += lin_load(a.bias, (size_t)a.N + n, a.type);
@@ -960,6 +1156,10 @@ cudaError_t lin_launch(void (*kernel)(KArgs...), unsigned grid, unsigned block, 
     return cudaLaunchKernelEx(&lc, kernel, static_cast<KArgs>(args)...);
 }
 
+// Rows of x in one copy.  With fewer than 128 tokens the other rows of the tile's operand
+// keep whatever shared memory held: their sums go to accumulator rows that nobody reads.
+int lin_box_rows(int T) { return T >= LG_BM ? LG_BM : (T + 7) / 8 * 8; }
+
 LinParams lin_params(const LinearArgs& a, int rows, int cols)
 {
     LinParams p = {};
@@ -979,6 +1179,7 @@ LinParams lin_params(const LinearArgs& a, int rows, int cols)
     p.gated = a.gated;
     p.vec_y = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && (a.ldy * es) % 16 == 0;
     p.vec_r = reinterpret_cast<uintptr_t>(a.residual) % 16 == 0 && (a.ldr * es) % 16 == 0;
+    p.x_rows = lin_box_rows(a.T);
     p.mt = (a.T + rows - 1) / rows;
     p.nt = (a.N + cols - 1) / cols;
     p.w_evict_first = p.mt == 1;
@@ -995,10 +1196,11 @@ cudaError_t launch_tiles(const LinearArgs& a, int dev, cudaStream_t s)
     if (e != cudaSuccess) return e;
     CUtensorMap tx, tw;
     const uint64_t wrows = (uint64_t)a.N * (a.gated ? 2 : 1);
-    if (!lin_tmap(&tx, a.x, a.type, a.K, a.T, a.ldx, LG_BM) || !lin_tmap(&tw, a.w, a.type, a.K, wrows, a.ldw, BN / 2))
+    if (!lin_tmap(&tx, a.x, a.type, a.K, a.T, a.ldx, lin_box_rows(a.T)) || !lin_tmap(&tw, a.w, a.type, a.K, wrows, a.ldw, BN / 2))
         return cudaErrorInvalidValue;
     const LinParams p = lin_params(a, Cfg::ROWS, a.gated ? BN / 2 : BN);
     const long long tiles = (long long)p.mt * p.nt;
+    if (tiles >= (1LL << 29)) return cudaErrorInvalidValue;  // (y would not fit any memory)
     long long units = lin_sm_count(dev);
     if (PAIR) {
         // co-resident pairs: both CTAs of a pair need a free SM of one GPC
@@ -1007,7 +1209,7 @@ cudaError_t launch_tiles(const LinearArgs& a, int dev, cudaStream_t s)
         if (units <= 0) {
             cudaLaunchConfig_t q = {};
             q.gridDim = dim3(2 * (lin_sm_count(dev) / 2));
-            q.blockDim = dim3(LG_THREADS);
+            q.blockDim = dim3(Cfg::THREADS);
             q.dynamicSmemBytes = lin_smem_bytes<PAIR, BN>();
             cudaLaunchAttribute ca;
             ca.id = cudaLaunchAttributeClusterDimension;
@@ -1026,40 +1228,90 @@ cudaError_t launch_tiles(const LinearArgs& a, int dev, cudaStream_t s)
         }
     }
     const unsigned grid = (unsigned)(tiles < units ? tiles : units) * (PAIR ? 2 : 1);
-    return lin_launch(kernel, grid, LG_THREADS, lin_smem_bytes<PAIR, BN>(), PAIR ? 2 : 0, s, tx, tw, p);
+    return lin_launch(kernel, grid, Cfg::THREADS, lin_smem_bytes<PAIR, BN>(), PAIR ? 2 : 0, s, tx, tw, p);
 }
 
-cudaError_t launch_split(const LinearArgs& a, int S, int dev, cudaStream_t s)
+template <int S, int BN>
+cudaError_t launch_split_as(const LinearArgs& a, int dev, cudaStream_t s)
 {
     static bool done[64] = {false};
-    cudaError_t e = lin_smem_attr(linear_split_kernel, LS_SMEM, done, dev);
+    auto* kernel = linear_split_kernel<S, BN>;
+    cudaError_t e = lin_smem_attr(kernel, SplitCfg<S, BN>::SMEM, done, dev);
     if (e != cudaSuccess) return e;
     CUtensorMap tx, tw;
     const uint64_t wrows = (uint64_t)a.N * (a.gated ? 2 : 1);
-    if (!lin_tmap(&tx, a.x, a.type, a.K, a.T, a.ldx, LG_BM) || !lin_tmap(&tw, a.w, a.type, a.K, wrows, a.ldw, LS_BN / 2))
+    if (!lin_tmap(&tx, a.x, a.type, a.K, a.T, a.ldx, lin_box_rows(a.T)) ||
+        !lin_tmap(&tw, a.w, a.type, a.K, wrows, a.ldw, BN / 2))
         return cudaErrorInvalidValue;
-    const LinParams p = lin_params(a, LG_BM, a.gated ? LS_BN / 2 : LS_BN);
+    const LinParams p = lin_params(a, LG_BM, a.gated ? BN / 2 : BN);
     const long long tiles = (long long)p.mt * p.nt;
-    return lin_launch(linear_split_kernel, (unsigned)(tiles * S), LG_THREADS, LS_SMEM, (unsigned)S, s, tx, tw, p, S);
+    if (tiles >= (1LL << 27)) return cudaErrorInvalidValue;  // (y would not fit any memory)
+    return lin_launch(kernel, (unsigned)(tiles * S), LS_THREADS, SplitCfg<S, BN>::SMEM, (unsigned)S, s, tx, tw, p);
+}
+
+cudaError_t launch_split(const LinearArgs& a, int S, int bn, int dev, cudaStream_t s)
+{
+    if (S == 8) return launch_split_as<8, 128>(a, dev, s);
+    if (S == 4) return bn == 64 ? launch_split_as<4, 64>(a, dev, s) : launch_split_as<4, 128>(a, dev, s);
+    return bn == 64 ? launch_split_as<2, 64>(a, dev, s) : launch_split_as<2, 128>(a, dev, s);
 }
 
 template <bool BF16, int MT>
-cudaError_t launch_few_rows(const LinearArgs& a, cudaStream_t s)
+cudaError_t launch_few_rows(const LinearArgs& a, int sms, cudaStream_t s)
 {
     const int rows = a.gated ? 16 : 16 * MT;
     const unsigned grid = (unsigned)((a.N + rows - 1) / rows);
-    if (a.T <= 8) return lin_launch(linear_few_kernel<BF16, MT, 1>, grid, LF_WARPS * 32, 0, 0, s, a);
-    return lin_launch(linear_few_kernel<BF16, MT, 2>, grid, LF_WARPS * 32, 0, 0, s, a);
+    const bool many = grid > (unsigned)sms;  // two blocks of 8 warps per SM, or one of 16
+    if (a.T <= 8)
+        return many ? lin_launch(linear_few_kernel<BF16, MT, 1, 8>, grid, 256, 0, 0, s, a)
+                    : lin_launch(linear_few_kernel<BF16, MT, 1, 16>, grid, 512, 0, 0, s, a);
+    return many ? lin_launch(linear_few_kernel<BF16, MT, 2, 8>, grid, 256, 0, 0, s, a)
+                : lin_launch(linear_few_kernel<BF16, MT, 2, 16>, grid, 512, 0, 0, s, a);
 }
 
-cudaError_t launch_few(const LinearArgs& a, int mt, cudaStream_t s)
+cudaError_t launch_few(const LinearArgs& a, int mt, int sms, cudaStream_t s)
 {
-    if (a.type == MOE_DT_BF16) return mt == 2 ? launch_few_rows<true, 2>(a, s) : launch_few_rows<true, 1>(a, s);
-    return mt == 2 ? launch_few_rows<false, 2>(a, s) : launch_few_rows<false, 1>(a, s);
+    if (a.type == MOE_DT_BF16) return mt == 2 ? launch_few_rows<true, 2>(a, sms, s) : launch_few_rows<true, 1>(a, sms, s);
+    return mt == 2 ? launch_few_rows<false, 2>(a, sms, s) : launch_few_rows<false, 1>(a, sms, s);
 }
 
-// MOE_LINEAR_TILE=pair|wide|narrow|split1|split2|split4|split8|few forces a kernel where
-// it can run (few: up to 16 tokens; splitS: as many k blocks as CTAs).
+// How to share out k when the 128 x 128 tiles leave SMs idle.  The model, in ns: a k block
+// costs 160 (whole tiles), 200 (split, 128 columns) or 130 (64 columns: half the bytes) and
+// the exchange of partial sums 800 and its bytes at 21 per ns, the rate measured for
+// distributed shared memory.  `cap` is how many CTAs run at once: a cluster of 8 (4, 2)
+// finds room 15 (33, 74) times.  Against the measured order: 128 x 2048 -> 2048: <4, 64>
+// 8.2 us, <4, 128> 10.5, <2, 64> 9.7, whole tiles 11.1; 17 x 7168 -> 256: <8, 128> 8.3,
+// <4, 64> 10.9; 512 x 2048 -> 2048: whole tiles 11.3, <2, 128> 13.4.
+struct SplitChoice {
+    int S, bn;
+};
+SplitChoice choose_split(int T, long long wrows, int nk, int sms)
+{
+    static const struct {
+        int S, bn, cap;
+    } opt[] = {{1, 128, 148}, {2, 128, 148}, {4, 128, 132}, {8, 128, 120}, {2, 64, 148}, {4, 64, 132}};
+    SplitChoice best = {1, 128};
+    double least = 1e30;
+    const int rows = T >= LG_BM ? LG_BM : (T + 31) / 32 * 32;
+    for (const auto& o : opt) {
+        if (o.S > nk) continue;
+        const long long tiles = (long long)((T + LG_BM - 1) / LG_BM) * ((wrows + o.bn - 1) / o.bn);
+        const long long cap = (long long)o.cap * sms / 148 > o.S ? (long long)o.cap * sms / 148 : o.S;
+        const double waves = (double)((tiles * o.S + cap - 1) / cap);
+        const double kb = o.S == 1 ? 160.0 : (o.bn == 64 ? 130.0 : 200.0);
+        const double exchange = o.S == 1 ? 0.0 : 800.0 + rows * o.bn * 4.0 * (o.S - 1) / o.S / 21.0;
+        const double cost = waves * ((nk + o.S - 1) / o.S * kb + exchange);
+        if (cost < least) {
+            least = cost;
+            best = {o.S, o.bn};
+        }
+    }
+    return best;
+}
+
+// MOE_LINEAR_TILE=pair|wide|narrow|split2|split4|split8|split2n|split4n|few forces a kernel where
+// it can run (few: up to 16 tokens; splitS: as many k blocks as
+// CTAs; n: 64 columns per tile).
 const char* lin_forced()
 {
 #ifdef MOE_LINEAR_TUNE
@@ -1082,26 +1334,29 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s)
     const int few_mt = a.gated || wrows >= 32LL * 2 * sms ? 2 : 1;
     const long long mt = (a.T + LG_BM - 1) / LG_BM, nt128 = (wrows + 127) / 128;
     if (const char* f = lin_forced()) {
-        if (!strcmp(f, "few") && a.T <= 16) return launch_few(a, few_mt, s);
+        if (!strcmp(f, "few") && a.T <= 16) return launch_few(a, few_mt, sms, s);
         if (!strcmp(f, "pair")) return launch_tiles<1, 256>(a, dev, s);
         if (!strcmp(f, "wide")) return launch_tiles<0, 256>(a, dev, s);
         if (!strcmp(f, "narrow")) return launch_tiles<0, 128>(a, dev, s);
-        if (!strncmp(f, "split", 5) && f[5] >= '1' && f[5] <= '8' && mt * nt128 * 8 < (1LL << 31)) {
+        if (!strncmp(f, "split", 5) && f[5] >= '2' && f[5] <= '8') {
             int S = f[5] - '0';
             while (S > nk || (S & (S - 1))) S--;
-            return launch_split(a, S, dev, s);
+            if (S > 1) return launch_split(a, S, strstr(f, "n") ? 64 : 128, dev, s);
         }
     }
-    if (a.T <= 16) return launch_few(a, few_mt, s);
-    const long long t128 = mt * nt128;
-    if (2 * t128 <= sms) {
-        int S = 8;
-        while (S > 1 && (t128 * S > sms || S > nk)) S >>= 1;
-        return launch_split(a, S, dev, s);
-    }
-    if (t128 <= sms) return launch_tiles<0, 128>(a, dev, s);
-    if (t128 <= 4 * sms) return launch_tiles<0, 256>(a, dev, s);
-    return launch_tiles<1, 256>(a, dev, s);
+    // Few tokens.  Measured (us, few / the best of the others): 8 x 2048 -> 2048 4.3 / 6.0,
+    // 8 x 8192 -> 2048 9.1 / 13, gated 8 x 4096 -> 14336 40.0 / 40.6.  With two blocks of
+    // tokens the registers hold less of w on its way: 16 x 2048 -> 2048 5.2 / 5.8, but
+    // 16 x 8192 -> 2048 12.6 / 10.9, 16 x 4096 -> 16384 34 / 26, gated 16 x 2048 -> 8192 19 / 14.
+    if (a.T <= 8 || (a.T <= 16 && !a.gated && a.N <= 16 * sms && a.K <= 4096)) return launch_few(a, few_mt, sms, s);
+    // At most one wave of 128 x 128 tiles: those, or smaller ones with k split, whichever
+    // the model says; else 256 x 256 over CTA pairs, or 128 x 256 where a pair's second half
+    // would be empty.  Measured (us, pair / wide / narrow): 2048 x 2048 -> 2048 16.7 / 16.9 /
+    // 19.1, gated 512 x 2048 -> 8192 28.7 / 31.8 / 36, gated 128 x 4096 -> 14336 53 / 43 / 47.
+    if (mt * nt128 > sms) return a.T > LG_BM ? launch_tiles<1, 256>(a, dev, s) : launch_tiles<0, 256>(a, dev, s);
+    const SplitChoice c = choose_split(a.T, wrows, nk, sms);
+    if (c.S > 1) return launch_split(a, c.S, c.bn, dev, s);
+    return launch_tiles<0, 128>(a, dev, s);
 }
 
 }  // namespace moe
