@@ -42,7 +42,24 @@ template <int ACT>
 __device__ __forceinline__ float lin_act1(float z)
 {
     if (ACT == MOE_ACT_RELU) return z < 0.0f ? 0.0f : z;  // NaN stays
-    if (ACT == MOE_ACT_GELU) return z * normcdff(z);
+    if (ACT == MOE_ACT_GELU) {
+        // z Phi(z), with Phi(-|z|) = erfc(|z| / sqrt 2) / 2 by the Chebyshev fit of Press et
+        // al., Numerical Recipes (erfcc): erfc(x) = t exp(-x^2 + P(t)), t = 1 / (1 + x / 2),
+        // relative error below 1.2e-7 for every x >= 0
+        const float t = __fdividef(1.0f, fmaf(0.35355339f, fabsf(z), 1.0f));
+        float e = 0.17087277f;
+        e = fmaf(e, t, -0.82215223f);
+        e = fmaf(e, t, 1.48851587f);
+        e = fmaf(e, t, -1.13520398f);
+        e = fmaf(e, t, 0.27886807f);
+        e = fmaf(e, t, -0.18628806f);
+        e = fmaf(e, t, 0.09678418f);
+        e = fmaf(e, t, 0.37409196f);
+        e = fmaf(e, t, 1.00002368f);
+        e = fmaf(e, t, -1.26551223f);
+        const float q = 0.5f * t * __expf(fmaf(-0.5f * z, z, e));
+        return z * (z > 0.0f ? 1.0f - q : q);
+    }
     if (ACT == MOE_ACT_GELU_TANH) {
         // 0.5 z (1 + tanh(u)) = z / (1 + exp(-2u)), u = sqrt(2/pi) (z + 0.044715 z^3)
         const float u2 = 1.5957691216057308f * (z + 0.044715f * z * z * z);
@@ -211,6 +228,11 @@ constexpr int LG_A_BYTES = LG_BM * LG_BK * 2;  // 16 KB
 constexpr int LG_EPI_WARPS = 8;                // two per TMEM lane quarter, taking chunks in turn
 constexpr int LG_THREADS = 64 + 32 * LG_EPI_WARPS;  // narrow tiles: one warp more
 constexpr int LG_MAX_STAGES = 8;
+// The tensor cores add in fp32 but cut off instead of rounding, always towards zero: over
+// 2048 products y is 2.5e-6 of its size off (rounded sums: 0.8e-6), and in proportion over
+// more.  A 16-bit y does not show it; for an fp32 one the accumulator is emptied into
+// registers, which round, every 8 k blocks (512 products).
+constexpr int LG_SEGMENT = 8;
 constexpr int LG_GROUP_M = 8;                  // m tiles that run together over all n tiles
 
 // PAIR: a 2-CTA cluster runs 256 x 256 tiles with cta_group::2 UMMAs; each CTA stages its
@@ -303,74 +325,56 @@ __device__ __forceinline__ void lin_add_bias(const LinParams& p, int lane, int n
     for (int c = 0; c < 32; c++) v[c] += __shfl_sync(0xffffffffu, b, c);
 }
 
-// One warp's 32 rows x `cols` outputs of a tile: accumulators from TMEM (tbase; the up
-// sums of a gated tile `up` columns further), bias, activation, gate, residual, store.
-// A chunk of 32 columns at a time (every other one: `half`), straight-line: an SM runs two
-// such warps per scheduler, so most dependent instructions are waited for.  Stores and residual loads go through
-// shared memory, so that each instruction covers whole 64-byte row segments.
+// Where one warp's part of a tile goes: 32 rows from row0 (`rows` of them exist), `valid`
+// columns from col0.
+struct LinWarpTile {
+    uint8_t* stg;
+    int lane, row0, rows, col0, valid;
+};
+
+// Stores 32 columns from column j of the part: v[c] belongs to this lane's row.  Straight
+// line: an SM runs two such warps per scheduler, so most dependent instructions are waited
+// for.  Stores and residual loads go through shared memory, so that each instruction covers
+// whole 64-byte row segments.
 template <int OT>
-__device__ __forceinline__ void lin_epilogue(const LinParams& p, uint32_t tbase, int up, uint8_t* stg, int lane, int row0,
-                                             int rows, int col0, int cols, int half)
-{
+struct LinChunk {
     typedef typename LinOut<OT>::T TO;
-    constexpr int HALVES = OT == MOE_DT_FLOAT ? 2 : 1;  // 64-byte pieces of a 32-column chunk
-    constexpr int HC = 32 / HALVES;                     // columns per piece
-    constexpr int E16 = 16 / (int)sizeof(TO);           // elements of 16 bytes
-    uint4* const mine = reinterpret_cast<uint4*>(stg + lane * LG_STG_ROW);
-    // the transposed view: lane -> rows r0 + 8 i, 16-byte piece c0 of the 64
-    const int r0 = lane >> 2, c0 = lane & 3;
-    const uint4* const trans = reinterpret_cast<const uint4*>(stg + r0 * LG_STG_ROW + c0 * 16);
-    const bool aligned = p.vec_y && (!p.residual || p.vec_r);
-    TO* const y = static_cast<TO*>(p.y) + (size_t)row0 * p.ldy + col0;
-    const TO* const res = p.residual ? static_cast<const TO*>(p.residual) + (size_t)row0 * p.ldr + col0 : nullptr;
-    const int valid = min(cols, p.N - col0);
-#pragma unroll 1
-    for (int j = 32 * half; j < valid; j += 64) {
-        uint32_t a[32];
-        float v[32];
-        tmem_ld_32x32b_x32(tbase + j, a);
-        const bool fast = aligned && j + 32 <= valid;
-        uint4 rq[HALVES * 4];
-        if (res && fast) {
+    static constexpr int HALVES = OT == MOE_DT_FLOAT ? 2 : 1;  // 64-byte pieces of 32 columns
+    static constexpr int HC = 32 / HALVES;                     // columns per piece
+    static constexpr int E16 = 16 / (int)sizeof(TO);           // elements of 16 bytes
+    uint4 rq[HALVES * 4];
+    bool fast;
+
+    // rows r0 + 8 i, 16-byte piece c0 of the 64, are this lane's in the transposed view
+    __device__ __forceinline__ void load_residual(const LinParams& p, const LinWarpTile& w, int j)
+    {
+        fast = p.vec_y && (!p.residual || p.vec_r) && j + 32 <= w.valid;
+        if (p.residual && fast) {
+            const int r0 = w.lane >> 2, c0 = w.lane & 3;
+            const TO* res = static_cast<const TO*>(p.residual) + (size_t)w.row0 * p.ldr + w.col0 + j + c0 * E16;
 #pragma unroll
             for (int h = 0; h < HALVES; h++)
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-                    if (r0 + 8 * i < rows)
-                        rq[h * 4 + i] = *reinterpret_cast<const uint4*>(res + (size_t)(r0 + 8 * i) * p.ldr + j + h * HC +
-                                                                         c0 * E16);
+                    if (r0 + 8 * i < w.rows)
+                        rq[h * 4 + i] = *reinterpret_cast<const uint4*>(res + (size_t)(r0 + 8 * i) * p.ldr + h * HC);
         }
-        if (p.gated) {
-            uint32_t b[32];
-            float u[32];
-            tmem_ld_32x32b_x32(tbase + up + j, b);
-            tmem_ld_wait();
-#pragma unroll
-            for (int c = 0; c < 32; c++) {
-                v[c] = __uint_as_float(a[c]);
-                u[c] = __uint_as_float(b[c]);
-            }
-            if (p.bias) {
-                lin_add_bias(p, lane, col0 + j, 0, v);
-                lin_add_bias(p, lane, col0 + j, p.N, u);
-            }
-            lin_act(v, p.act);
-#pragma unroll
-            for (int c = 0; c < 32; c++) v[c] *= u[c];
-        } else {
-            tmem_ld_wait();
-#pragma unroll
-            for (int c = 0; c < 32; c++) v[c] = __uint_as_float(a[c]);
-            if (p.bias) lin_add_bias(p, lane, col0 + j, 0, v);
-            lin_act(v, p.act);
-        }
+    }
+
+    __device__ __forceinline__ void store(const LinParams& p, const LinWarpTile& w, int j, float (&v)[32])
+    {
+        uint8_t* const stg = w.stg;
+        uint4* const mine = reinterpret_cast<uint4*>(stg + w.lane * LG_STG_ROW);
+        TO* const y = static_cast<TO*>(p.y) + (size_t)w.row0 * p.ldy + w.col0 + j;
         if (fast) {
+            const int r0 = w.lane >> 2, c0 = w.lane & 3;
+            uint4* const trans = reinterpret_cast<uint4*>(stg + r0 * LG_STG_ROW + c0 * 16);
+            constexpr int STEP = 8 * LG_STG_ROW / 16;
 #pragma unroll
             for (int h = 0; h < HALVES; h++) {
-                if (res) {
+                if (p.residual) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        *reinterpret_cast<uint4*>(stg + (r0 + 8 * i) * LG_STG_ROW + c0 * 16) = rq[h * 4 + i];
+                    for (int i = 0; i < 4; i++) trans[i * STEP] = rq[h * 4 + i];
                     __syncwarp();
 #pragma unroll
                     for (int i = 0; i < 4; i++) lin_add16<OT>(v + h * HC + i * E16, mine[i]);
@@ -381,43 +385,119 @@ __device__ __forceinline__ void lin_epilogue(const LinParams& p, uint32_t tbase,
                 __syncwarp();
                 uint4 o[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) o[i] = trans[i * 8 * LG_STG_ROW / 16];
+                for (int i = 0; i < 4; i++) o[i] = trans[i * STEP];
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-                    if (r0 + 8 * i < rows)
-                        *reinterpret_cast<uint4*>(y + (size_t)(r0 + 8 * i) * p.ldy + j + h * HC + c0 * E16) = o[i];
+                    if (r0 + 8 * i < w.rows)
+                        *reinterpret_cast<uint4*>(y + (size_t)(r0 + 8 * i) * p.ldy + h * HC + c0 * E16) = o[i];
                 __syncwarp();
             }
         } else {
-            // rows off 16-byte boundaries, or the last columns: half a warp per row, an
-            // element per lane, in fp32 through the staging rows
-            const int rr = lane >> 4, c = lane & 15;
+            // Rows off 16-byte boundaries, or the last columns: an element per lane, so that
+            // an instruction still covers whole 64-byte segments (two half rows of them, as
+            // this once did, took 1.5 times as long: L2 merges every partial sector).
+            constexpr int RPI = 32 / HC;  // rows per instruction
+            const int rr = w.lane / HC, c = w.lane % HC;
+            const TO* const res =
+                p.residual ? static_cast<const TO*>(p.residual) + (size_t)w.row0 * p.ldr + w.col0 + j : nullptr;
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
+            for (int h = 0; h < HALVES; h++) {
+                const bool in = j + h * HC + c < w.valid;
+                if (res) {
+                    // every load without a condition (clamped to what exists), all at once
+                    const TO* const src = res + (in ? h * HC + c : 0);
+                    TO a[32 / RPI];
 #pragma unroll
-                for (int i = 0; i < 4; i++) mine[i] = lin_pack16<MOE_DT_FLOAT>(v + h * 16 + i * 4);
+                    for (int i = 0; i < 32 / RPI; i++) a[i] = src[(size_t)min(i * RPI + rr, w.rows - 1) * p.ldr];
+#pragma unroll
+                    for (int i = 0; i < 32 / RPI; i++)
+                        reinterpret_cast<TO*>(stg + (i * RPI + rr) * LG_STG_ROW)[c] = a[i];
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 4; i++) lin_add16<OT>(v + h * HC + i * E16, mine[i]);
+                    __syncwarp();
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) mine[i] = lin_pack16<OT>(v + h * HC + i * E16);
                 __syncwarp();
-                const int n = j + h * 16 + c;
-                if (n < valid) {
+                if (in) {
 #pragma unroll 8
-                    for (int r = rr; r < rows; r += 2) {
-                        float f = *reinterpret_cast<const float*>(stg + r * LG_STG_ROW + c * 4);
-                        if (res) f += LinOut<OT>::from(res[(size_t)r * p.ldr + n]);
-                        y[(size_t)r * p.ldy + n] = LinOut<OT>::to(f);
-                    }
+                    for (int r = rr; r < w.rows; r += RPI)
+                        y[(size_t)r * p.ldy + h * HC + c] = reinterpret_cast<const TO*>(stg + r * LG_STG_ROW)[c];
                 }
                 __syncwarp();
             }
         }
     }
+};
+
+// Brings the residual of a warp's rows on its way while the products still run: a lane per
+// row, the lines that its columns touch (the two warps of a quarter take every other one).
+__device__ __forceinline__ void lin_prefetch_residual(const LinParams& p, const LinWarpTile& w, int half)
+{
+    if (!p.residual || w.lane >= w.rows) return;
+    const size_t es = p.otype == MOE_DT_FLOAT ? 4 : 2;
+    const uintptr_t row = reinterpret_cast<uintptr_t>(p.residual) + ((size_t)(w.row0 + w.lane) * p.ldr + w.col0) * es;
+    const uintptr_t end = row + (size_t)w.valid * es;
+    for (uintptr_t a = (row & ~(uintptr_t)127) + 128 * half; a < end; a += 256)
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(a < row ? row : a));
 }
 
-template <int PAIR, int BN>
+__device__ __forceinline__ void lin_tmem_load(uint32_t taddr, float (&v)[32])
+{
+    uint32_t a[32];
+    tmem_ld_32x32b_x32(taddr, a);
+    tmem_ld_wait();
+#pragma unroll
+    for (int c = 0; c < 32; c++) v[c] = __uint_as_float(a[c]);
+}
+
+// A warp's part of a 16-bit tile, every other chunk of 32 columns (`half`): sums from TMEM
+// (tbase; the up sums of a gated tile `up` columns further), bias, activation, gate,
+// residual, store.
+template <int OT>
+__device__ __forceinline__ void lin_epilogue(const LinParams& p, uint32_t tbase, int up, const LinWarpTile& w, int half)
+{
+#pragma unroll 1
+    for (int j = 32 * half; j < w.valid; j += 64) {
+        float v[32];
+        LinChunk<OT> chunk;
+        chunk.load_residual(p, w, j);
+        if (p.gated) {
+            float u[32];
+            uint32_t a[32], b[32];
+            tmem_ld_32x32b_x32(tbase + j, a);
+            tmem_ld_32x32b_x32(tbase + up + j, b);
+            tmem_ld_wait();
+#pragma unroll
+            for (int c = 0; c < 32; c++) {
+                v[c] = __uint_as_float(a[c]);
+                u[c] = __uint_as_float(b[c]);
+            }
+            if (p.bias) {
+                lin_add_bias(p, w.lane, w.col0 + j, 0, v);
+                lin_add_bias(p, w.lane, w.col0 + j, p.N, u);
+            }
+            lin_act(v, p.act);
+#pragma unroll
+            for (int c = 0; c < 32; c++) v[c] *= u[c];
+        } else {
+            lin_tmem_load(tbase + j, v);
+            if (p.bias) lin_add_bias(p, w.lane, w.col0 + j, 0, v);
+            lin_act(v, p.act);
+        }
+        chunk.store(p, w, j, v);
+    }
+}
+
+// F32: y is fp32, and the sums go through registers every LG_SEGMENT k blocks.
+template <int PAIR, int BN, bool F32>
 __global__ void __launch_bounds__((LinCfg<PAIR, BN>::THREADS), 1)
 linear_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
                    const LinParams p)
 {
     using Cfg = LinCfg<PAIR, BN>;
+    static_assert(!F32 || (BN == 128 && !PAIR), "a warp holds two chunks of sums");
     constexpr int STAGES = Cfg::STAGES;
     constexpr int STAGE_BYTES = Cfg::STAGE_BYTES;
     constexpr int ROWS = Cfg::ROWS;
@@ -539,46 +619,51 @@ linear_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
         // ---------------------------------------------------------------- UMMA issuer
         if (leader && elect_one()) {
             const uint32_t idesc = lin_idesc(ROWS, BN, p.type == MOE_DT_BF16);
+            const int seg = F32 ? LG_SEGMENT : nk;
             uint32_t it = 0, lt = 0;
             bool ok = true;
-            for (int tile = unit; ok && tile < total; tile += nunits, lt++) {
-                const uint32_t acc = lt & 1u;
-                const uint32_t tpar = ((lt >> 1) & 1u) ^ 1u;
-                if (!(lin_wait<PAIR != 0>(smem_u32(&tail->tempty[acc]), tpar, err, MOE_DEV_WAIT_TIMEOUT_MMA, abort_flag)))
-                    break;
-                tc_fence_after();
-                const uint32_t d = tmem_base + acc * BN;
-                for (int kb = 0; kb < nk; kb += KPS, it++) {
-                    const int s = it % STAGES;
-                    if (!lin_wait<PAIR != 0>(smem_u32(&tail->full[s]), (it / STAGES) & 1u, err,
-                                                       MOE_DEV_WAIT_TIMEOUT_MMA, abort_flag)) {
+            for (int tile = unit; ok && tile < total; tile += nunits) {
+                for (int k0 = 0; ok && k0 < nk; k0 += seg, lt++) {
+                    const int k1 = min(k0 + seg, nk);
+                    const uint32_t acc = lt & 1u;
+                    if (!lin_wait<PAIR != 0>(smem_u32(&tail->tempty[acc]), ((lt >> 1) & 1u) ^ 1u, err,
+                                             MOE_DEV_WAIT_TIMEOUT_MMA, abort_flag)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
+                    const uint32_t d = tmem_base + acc * BN;
+                    for (int kb = k0; kb < k1; kb += KPS, it++) {
+                        const int s = it % STAGES;
+                        if (!lin_wait<PAIR != 0>(smem_u32(&tail->full[s]), (it / STAGES) & 1u, err,
+                                                 MOE_DEV_WAIT_TIMEOUT_MMA, abort_flag)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
 #pragma unroll
-                    for (int i = 0; i < KPS; i++) {
-                        if (kb + i >= nk) break;
-                        const uint32_t a_addr = smem_u32(smem + s * STAGE_BYTES + i * Cfg::KB_BYTES);
-                        const uint32_t b_addr = a_addr + LG_A_BYTES;
+                        for (int i = 0; i < KPS; i++) {
+                            if (kb + i >= k1) break;
+                            const uint32_t a_addr = smem_u32(smem + s * STAGE_BYTES + i * Cfg::KB_BYTES);
+                            const uint32_t b_addr = a_addr + LG_A_BYTES;
 #pragma unroll
-                        for (int k = 0; k < LG_BK / 16; k++) {
-                            // k advances by 16 elements = 32 bytes inside the swizzle row
-                            const uint64_t da = umma_desc_sw128(a_addr + k * 32), db = umma_desc_sw128(b_addr + k * 32);
-                            if (PAIR)
-                                umma_f16_ss_pair(d, da, db, idesc, (kb | i | k) != 0);
-                            else
-                                umma_f16_ss(d, da, db, idesc, (kb | i | k) != 0);
+                            for (int k = 0; k < LG_BK / 16; k++) {
+                                // k advances by 16 elements = 32 bytes inside the swizzle row
+                                const uint64_t da = umma_desc_sw128(a_addr + k * 32), db = umma_desc_sw128(b_addr + k * 32);
+                                if (PAIR)
+                                    umma_f16_ss_pair(d, da, db, idesc, (kb - k0) | i | k);
+                                else
+                                    umma_f16_ss(d, da, db, idesc, (kb - k0) | i | k);
+                            }
+                        }
+                        if (PAIR) {
+                            umma_commit_pair(smem_u32(&tail->empty[s]));
+                            umma_commit_pair(mapa_shared(smem_u32(&tail->empty[s]), 1));
+                        } else {
+                            umma_commit(smem_u32(&tail->empty[s]));
                         }
                     }
-                    if (PAIR) {
-                        umma_commit_pair(smem_u32(&tail->empty[s]));
-                        umma_commit_pair(mapa_shared(smem_u32(&tail->empty[s]), 1));
-                    } else {
-                        umma_commit(smem_u32(&tail->empty[s]));
-                    }
-                }
-                if (ok) {
+                    if (!ok) break;
                     if (PAIR) {
                         umma_commit_pair(smem_u32(&tail->tfull[acc]));
                         umma_commit_pair(mapa_shared(smem_u32(&tail->tfull[acc]), 1));
@@ -607,29 +692,85 @@ linear_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
             lin_tile(p, tile, m, n);
             const uint32_t acc = lt & 1u;
             const uint32_t tpar = (lt >> 1) & 1u;
+            const int cols = p.gated ? BN / 2 : BN;
+            LinWarpTile w = {stg, lane, m * ROWS + (int)crank * LG_BM + q * 32, 0, n * cols, 0};
+            w.rows = min(32, p.T - w.row0);  // <= 0: none of this warp's rows exist
+            w.valid = min(cols, p.N - w.col0);
+            lin_prefetch_residual(p, w, half);
             if (!(lin_wait<PAIR != 0>(smem_u32(&tail->tfull[acc]), tpar, err, MOE_DEV_WAIT_TIMEOUT_EPI, abort_flag)))
                 break;
             tc_fence_after();
-            const int row0 = m * ROWS + (int)crank * LG_BM + q * 32;
-            const int rows = min(32, p.T - row0);  // <= 0: none of this warp's rows exist
-            const uint32_t tbase = tmem_base + acc * BN + ((uint32_t)(q * 32) << 16);
-            const int cols = p.gated ? BN / 2 : BN;
-            if (rows > 0) {
+            const uint32_t quarter = tmem_base + ((uint32_t)(q * 32) << 16);
+            if constexpr (F32) {
+                // The sums of this warp's two chunks (gated: gate and up of one), added up
+                // over the segments in fp32 registers; the accumulator of one segment is
+                // read while the next one's products run.
+                const int j0 = 32 * half, j1 = p.gated ? BN / 2 + j0 : j0 + 64;
+                float v[32], u[32];
+                bool ok = true;
+                for (int k0 = 0; k0 < nk; k0 += LG_SEGMENT, lt++) {
+                    const uint32_t acc = lt & 1u;
+                    if (k0 > 0 && !lin_wait<false>(smem_u32(&tail->tfull[acc]), (lt >> 1) & 1u, err,
+                                                   MOE_DEV_WAIT_TIMEOUT_EPI, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    if (k0 == 0) {
+                        lin_tmem_load(quarter + acc * BN + j0, v);
+                        lin_tmem_load(quarter + acc * BN + j1, u);
+                    } else {
+                        float a[32];
+                        lin_tmem_load(quarter + acc * BN + j0, a);
+#pragma unroll
+                        for (int c = 0; c < 32; c++) v[c] += a[c];
+                        lin_tmem_load(quarter + acc * BN + j1, a);
+#pragma unroll
+                        for (int c = 0; c < 32; c++) u[c] += a[c];
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(tempty0 + acc * (uint32_t)sizeof(uint64_t));
+                }
+                if (!ok) break;
+                lt--;  // the loop's step counts the last segment
+                if (w.rows > 0) {
+                    if (p.bias) {
+                        lin_add_bias(p, lane, w.col0 + j0, 0, v);
+                        lin_add_bias(p, lane, w.col0 + (p.gated ? j0 : j1), p.gated ? (size_t)p.N : 0, u);
+                    }
+                    lin_act(v, p.act);
+                    LinChunk<MOE_DT_FLOAT> chunk;
+                    if (p.gated) {
+#pragma unroll
+                        for (int c = 0; c < 32; c++) v[c] *= u[c];
+                    }
+                    if (j0 < w.valid) {
+                        chunk.load_residual(p, w, j0);
+                        chunk.store(p, w, j0, v);
+                    }
+                    if (!p.gated && j1 < w.valid) {
+                        lin_act(u, p.act);
+                        chunk.load_residual(p, w, j1);
+                        chunk.store(p, w, j1, u);
+                    }
+                }
+            } else if (w.rows > 0) {
                 if (p.otype == MOE_DT_FLOAT16)
-                    lin_epilogue<MOE_DT_FLOAT16>(p, tbase, BN / 2, stg, lane, row0, rows, n * cols, cols, half);
-                else if (p.otype == MOE_DT_BF16)
-                    lin_epilogue<MOE_DT_BF16>(p, tbase, BN / 2, stg, lane, row0, rows, n * cols, cols, half);
+                    lin_epilogue<MOE_DT_FLOAT16>(p, quarter + acc * BN, BN / 2, w, half);
                 else
-                    lin_epilogue<MOE_DT_FLOAT>(p, tbase, BN / 2, stg, lane, row0, rows, n * cols, cols, half);
+                    lin_epilogue<MOE_DT_BF16>(p, quarter + acc * BN, BN / 2, w, half);
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                const uint32_t bar = tempty0 + acc * (uint32_t)sizeof(uint64_t);
-                if (PAIR)
-                    mbar_arrive_cluster(bar);
-                else
-                    mbar_arrive(bar);
+            if (!F32) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    const uint32_t bar = tempty0 + acc * (uint32_t)sizeof(uint64_t);
+                    if (PAIR)
+                        mbar_arrive_cluster(bar);
+                    else
+                        mbar_arrive(bar);
+                }
             }
         }
     }
@@ -776,6 +917,12 @@ linear_split_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
     int* err = p.err ? p.err : &g_linear_err;
     const int rank = (int)cluster_ctarank();
     const int tile = (int)(blockIdx.x / S);
+    const int kb0 = (int)((long long)p.nk * rank / S), kb1 = (int)((long long)p.nk * (rank + 1) / S);
+    // an fp32 y: the sums of each `seg` k blocks have an accumulator of their own (see
+    // LG_SEGMENT; here as many as TMEM holds, added up when they are read)
+    const bool parts = p.otype == MOE_DT_FLOAT;
+    const uint32_t tmem_cols = parts ? 512 : BN;
+    const int seg = parts ? max(LG_SEGMENT, ((((kb1 - kb0) * BN + 511) / 512) + 1) & ~1) : kb1 - kb0;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < Cfg::STAGES; s++) {
@@ -791,7 +938,7 @@ linear_split_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
     }
     pdl_trigger();
     if (warp == 1) {
-        tmem_alloc(smem_u32(&tail->tmem_base), BN);
+        tmem_alloc(smem_u32(&tail->tmem_base), tmem_cols);
         tmem_relinquish();
     }
     int m, n;
@@ -807,7 +954,6 @@ linear_split_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
 
     const uint32_t tmem_base = tail->tmem_base;
     volatile int* abort_flag = &tail->abort_flag;
-    const int kb0 = (int)((long long)p.nk * rank / S), kb1 = (int)((long long)p.nk * (rank + 1) / S);
     const int cols = p.gated ? BN / 2 : BN;
 
     if (warp == 0 || warp == 6) {
@@ -864,6 +1010,8 @@ linear_split_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
                                                MOE_DEV_WAIT_TIMEOUT_MMA, abort_flag))
                     break;
                 tc_fence_after();
+                const int part = (kb - kb0) / seg, first = kb0 + part * seg;  // seg is even or the whole
+                const uint32_t d = tmem_base + part * BN;
 #pragma unroll
                 for (int i = 0; i < LS_KPS; i++) {
                     if (kb + i >= kb1) break;
@@ -871,8 +1019,8 @@ linear_split_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
                     const uint32_t b_addr = a_addr + LG_A_BYTES;
 #pragma unroll
                     for (int k = 0; k < LG_BK / 16; k++)
-                        umma_f16_ss(tmem_base, umma_desc_sw128(a_addr + k * 32), umma_desc_sw128(b_addr + k * 32), idesc,
-                                    (kb > kb0 || i > 0 || k > 0) ? 1u : 0u);
+                        umma_f16_ss(d, umma_desc_sw128(a_addr + k * 32), umma_desc_sw128(b_addr + k * 32), idesc,
+                                    (kb - first) | i | k);
                 }
                 umma_commit(smem_u32(&tail->empty[s]));
             }
@@ -887,9 +1035,14 @@ linear_split_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
             float* const mine = reinterpret_cast<float*>(smem) + (q * 32 + lane) * PITCH;
 #pragma unroll
             for (int j = 0; j < BN; j += 32) {
-                uint32_t a[32];
-                tmem_ld_32x32b_x32(tmem_base + ((uint32_t)(q * 32) << 16) + j, a);
-                tmem_ld_wait();
+                float a[32];
+                lin_tmem_load(tmem_base + ((uint32_t)(q * 32) << 16) + j, a);
+                for (int k0 = kb0 + seg, part = 1; k0 < kb1; k0 += seg, part++) {
+                    float more[32];
+                    lin_tmem_load(tmem_base + ((uint32_t)(q * 32) << 16) + part * BN + j, more);
+#pragma unroll
+                    for (int c = 0; c < 32; c++) a[c] += more[c];
+                }
 #pragma unroll
                 for (int c = 0; c < 32; c += 4) {
                     const int col = j + c;
@@ -897,8 +1050,7 @@ linear_split_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
                     const int d = p.gated ? col % (BN / 2) / (W / 2) : col / W;
                     const int off = p.gated ? col / (BN / 2) * (W / 2) + col % (BN / 2) % (W / 2) : col % W;
                     *reinterpret_cast<float4*>(mine + d * LG_BM * PITCH + off) =
-                        make_float4(__uint_as_float(a[c]), __uint_as_float(a[c + 1]), __uint_as_float(a[c + 2]),
-                                    __uint_as_float(a[c + 3]));
+                        make_float4(a[c], a[c + 1], a[c + 2], a[c + 3]);
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -919,7 +1071,7 @@ linear_split_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
     const bool arrived = *abort_flag == 0;
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem_base, BN);
+        tmem_dealloc(tmem_base, tmem_cols);
     }
     // no CTA leaves while its sums may still be read: all have arrived here once all have
     // received
@@ -972,9 +1124,9 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// k chunks of 32 in flight per warp: 160 to 256 bytes of w per lane
+// k chunks of 32 in flight per warp: 128 to 256 bytes of w per lane
 template <int MT, int NT>
-constexpr int lin_few_depth() { return MT == 2 ? (NT == 2 ? 3 : 4) : (NT == 2 ? 5 : 8); }
+constexpr int lin_few_depth() { return MT == 2 || NT == 2 ? 4 : 8; }
 
 template <bool BF16, int MT, int NT, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) linear_few_kernel(const LinearArgs a)
@@ -1024,6 +1176,7 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) linear_few_kernel(cons
 #pragma unroll
     for (int d = 0; d < D; d++) load(d, chunk_k(d));
     for (int c = 0; chunk_k(c) < a.K; c += D) {
+        float sum[MT][NT][4] = {};  // added up here, where sums are rounded (see LG_SEGMENT)
 #pragma unroll
         for (int d = 0; d < D; d++) {
 #pragma unroll
@@ -1031,11 +1184,17 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) linear_few_kernel(cons
 #pragma unroll
                 for (int j = 0; j < NT; j++) {
                     const uint4 lo = wa[d][i][0], hi = wa[d][i][1], b = xb[d][j];
-                    mma_16816<BF16>(acc[i][j], lo.x, hi.x, lo.y, hi.y, b.x, b.y);
-                    mma_16816<BF16>(acc[i][j], lo.z, hi.z, lo.w, hi.w, b.z, b.w);
+                    mma_16816<BF16>(sum[i][j], lo.x, hi.x, lo.y, hi.y, b.x, b.y);
+                    mma_16816<BF16>(sum[i][j], lo.z, hi.z, lo.w, hi.w, b.z, b.w);
                 }
             load(d, chunk_k(c + d + D));
         }
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int j = 0; j < NT; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[i][j][e] += sum[i][j][e];
     }
 #pragma unroll
     for (int i = 0; i < MT; i++)
@@ -1186,12 +1345,12 @@ LinParams lin_params(const LinearArgs& a, int rows, int cols)
     return p;
 }
 
-template <int PAIR, int BN>
+template <int PAIR, int BN, bool F32 = false>
 cudaError_t launch_tiles(const LinearArgs& a, int dev, cudaStream_t s)
 {
     using Cfg = LinCfg<PAIR, BN>;
     static bool done[64] = {false};
-    auto* kernel = linear_gemm_kernel<PAIR, BN>;
+    auto* kernel = linear_gemm_kernel<PAIR, BN, F32>;
     cudaError_t e = lin_smem_attr(kernel, lin_smem_bytes<PAIR, BN>(), done, dev);
     if (e != cudaSuccess) return e;
     CUtensorMap tx, tw;
@@ -1256,23 +1415,24 @@ cudaError_t launch_split(const LinearArgs& a, int S, int bn, int dev, cudaStream
     return bn == 64 ? launch_split_as<2, 64>(a, dev, s) : launch_split_as<2, 128>(a, dev, s);
 }
 
-template <bool BF16, int MT>
-cudaError_t launch_few_rows(const LinearArgs& a, int sms, cudaStream_t s)
+template <bool BF16, int MT, int NT>
+cudaError_t launch_few_as(const LinearArgs& a, int sms, cudaStream_t s)
 {
     const int rows = a.gated ? 16 : 16 * MT;
     const unsigned grid = (unsigned)((a.N + rows - 1) / rows);
-    const bool many = grid > (unsigned)sms;  // two blocks of 8 warps per SM, or one of 16
-    if (a.T <= 8)
-        return many ? lin_launch(linear_few_kernel<BF16, MT, 1, 8>, grid, 256, 0, 0, s, a)
-                    : lin_launch(linear_few_kernel<BF16, MT, 1, 16>, grid, 512, 0, 0, s, a);
-    return many ? lin_launch(linear_few_kernel<BF16, MT, 2, 8>, grid, 256, 0, 0, s, a)
-                : lin_launch(linear_few_kernel<BF16, MT, 2, 16>, grid, 512, 0, 0, s, a);
+    // two blocks of 8 warps per SM, or one of 16 where there is no second block
+    if (grid > (unsigned)sms) return lin_launch(linear_few_kernel<BF16, MT, NT, 8>, grid, 256, 0, 0, s, a);
+    return lin_launch(linear_few_kernel<BF16, MT, NT, 16>, grid, 512, 0, 0, s, a);
 }
 
-cudaError_t launch_few(const LinearArgs& a, int mt, int sms, cudaStream_t s)
+// At most 8 tokens, or 16 when not gated.  Two blocks of w rows per warp (MT = 2): gated, or
+// rows enough for two blocks on every SM even so.
+cudaError_t launch_few(const LinearArgs& a, int sms, cudaStream_t s)
 {
-    if (a.type == MOE_DT_BF16) return mt == 2 ? launch_few_rows<true, 2>(a, sms, s) : launch_few_rows<true, 1>(a, sms, s);
-    return mt == 2 ? launch_few_rows<false, 2>(a, sms, s) : launch_few_rows<false, 1>(a, sms, s);
+    const bool bf16 = a.type == MOE_DT_BF16;
+    if (a.T > 8) return bf16 ? launch_few_as<true, 1, 2>(a, sms, s) : launch_few_as<false, 1, 2>(a, sms, s);
+    if (a.gated || a.N >= 64LL * sms) return bf16 ? launch_few_as<true, 2, 1>(a, sms, s) : launch_few_as<false, 2, 1>(a, sms, s);
+    return bf16 ? launch_few_as<true, 1, 1>(a, sms, s) : launch_few_as<false, 1, 1>(a, sms, s);
 }
 
 // How to share out k when the 128 x 128 tiles leave SMs idle.  The model, in ns: a k block
@@ -1310,7 +1470,7 @@ SplitChoice choose_split(int T, long long wrows, int nk, int sms)
 }
 
 // MOE_LINEAR_TILE=pair|wide|narrow|split2|split4|split8|split2n|split4n|few forces a kernel where
-// it can run (few: up to 16 tokens; splitS: as many k blocks as
+// it can run (few: up to 16 tokens, gated 8; pair and wide: a 16-bit y; splitS: as many k blocks as
 // CTAs; n: 64 columns per tile).
 const char* lin_forced()
 {
@@ -1331,13 +1491,13 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s)
     const int sms = lin_sm_count(dev);
     const long long wrows = (long long)a.N * (a.gated ? 2 : 1);
     const int nk = (a.K + LG_BK - 1) / LG_BK;
-    const int few_mt = a.gated || wrows >= 32LL * 2 * sms ? 2 : 1;
+    const bool f32 = a.otype == MOE_DT_FLOAT;
     const long long mt = (a.T + LG_BM - 1) / LG_BM, nt128 = (wrows + 127) / 128;
     if (const char* f = lin_forced()) {
-        if (!strcmp(f, "few") && a.T <= 16) return launch_few(a, few_mt, sms, s);
-        if (!strcmp(f, "pair")) return launch_tiles<1, 256>(a, dev, s);
-        if (!strcmp(f, "wide")) return launch_tiles<0, 256>(a, dev, s);
-        if (!strcmp(f, "narrow")) return launch_tiles<0, 128>(a, dev, s);
+        if (!strcmp(f, "few") && (a.T <= 8 || (a.T <= 16 && !a.gated))) return launch_few(a, sms, s);
+        if (!strcmp(f, "pair") && !f32) return launch_tiles<1, 256>(a, dev, s);
+        if (!strcmp(f, "wide") && !f32) return launch_tiles<0, 256>(a, dev, s);
+        if (!strcmp(f, "narrow")) return f32 ? launch_tiles<0, 128, true>(a, dev, s) : launch_tiles<0, 128>(a, dev, s);
         if (!strncmp(f, "split", 5) && f[5] >= '2' && f[5] <= '8') {
             int S = f[5] - '0';
             while (S > nk || (S & (S - 1))) S--;
@@ -1346,17 +1506,19 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s)
     }
     // Few tokens.  Measured (us, few / the best of the others): 8 x 2048 -> 2048 4.3 / 6.0,
     // 8 x 8192 -> 2048 9.1 / 13, gated 8 x 4096 -> 14336 40.0 / 40.6.  With two blocks of
-    // tokens the registers hold less of w on its way: 16 x 2048 -> 2048 5.2 / 5.8, but
-    // 16 x 8192 -> 2048 12.6 / 10.9, 16 x 4096 -> 16384 34 / 26, gated 16 x 2048 -> 8192 19 / 14.
-    if (a.T <= 8 || (a.T <= 16 && !a.gated && a.N <= 16 * sms && a.K <= 4096)) return launch_few(a, few_mt, sms, s);
+    // tokens the registers hold less of w on its way: 16 x 2048 -> 2048 4.5 / 5.8,
+    // 16 x 8192 -> 2048 9.7 / 10.9, but 16 x 4096 -> 16384 34 / 26.
+    if (a.T <= 8 || (a.T <= 16 && !a.gated && a.N <= 16 * sms)) return launch_few(a, sms, s);
     // At most one wave of 128 x 128 tiles: those, or smaller ones with k split, whichever
     // the model says; else 256 x 256 over CTA pairs, or 128 x 256 where a pair's second half
     // would be empty.  Measured (us, pair / wide / narrow): 2048 x 2048 -> 2048 16.7 / 16.9 /
     // 19.1, gated 512 x 2048 -> 8192 28.7 / 31.8 / 36, gated 128 x 4096 -> 14336 53 / 43 / 47.
-    if (mt * nt128 > sms) return a.T > LG_BM ? launch_tiles<1, 256>(a, dev, s) : launch_tiles<0, 256>(a, dev, s);
+    // An fp32 y takes narrow tiles: their warps can hold its sums (see LG_SEGMENT).
+    if (mt * nt128 > sms && !f32) return a.T > LG_BM ? launch_tiles<1, 256>(a, dev, s) : launch_tiles<0, 256>(a, dev, s);
+    if (mt * nt128 > sms) return f32 ? launch_tiles<0, 128, true>(a, dev, s) : launch_tiles<0, 128>(a, dev, s);
     const SplitChoice c = choose_split(a.T, wrows, nk, sms);
     if (c.S > 1) return launch_split(a, c.S, c.bn, dev, s);
-    return launch_tiles<0, 128>(a, dev, s);
+    return f32 ? launch_tiles<0, 128, true>(a, dev, s) : launch_tiles<0, 128>(a, dev, s);
 }
 
 }  // namespace moe
