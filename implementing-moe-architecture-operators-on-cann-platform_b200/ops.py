@@ -233,29 +233,42 @@ SCORE_FUNCS = {"softmax": 0, "sigmoid": 1}
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4, "sigmoid": 5}
 
 
-def _dtype_codes():
-    """torch dtype -> MOE_DT_* code (include/moe_ops.h)."""
-    global _codes
-    if _codes is None:
+class _Cuda:
+    """What every call needs from torch, looked up once."""
+
+    def __init__(self):
         torch = _torch()
-        _codes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 27}
-    return _codes
+        self.Tensor, self.empty = torch.Tensor, torch.empty
+        self.codes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 27}  # MOE_DT_* (include/moe_ops.h)
+        self.f32, self.f16, self.i32 = torch.float32, torch.float16, torch.int32
+        self.device = torch.cuda.device
+        self.current_device = torch.cuda.current_device
+        # the handle of a device's current stream, without building a Stream object
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        self.stream = raw or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-_codes = None
+_cuda_state = None
 
 
-def _rows(t, name, rows, cols, dtype, like):
-    """The row stride of a [rows, cols] CUDA matrix whose rows are contiguous (0 for a
-    single row); raises MoeError on anything else."""
-    if t.device != like.device:
-        raise MoeError(-1, f"{name} must be on {like.device} (no CPU fallback), got {t.device}")
+def _cu() -> _Cuda:
+    global _cuda_state
+    if _cuda_state is None:
+        _cuda_state = _Cuda()
+    return _cuda_state
+
+
+def _rows(t, name, rows, cols, dtype, dev):
+    """The row stride of a [rows, cols] matrix on `dev` whose rows are contiguous; raises
+    MoeError on anything else."""
+    if t.dtype is dtype and t.device == dev and t.shape == (rows, cols) and t.is_contiguous():
+        return cols
+    if t.device != dev:
+        raise MoeError(-1, f"{name} must be on {dev} (no CPU fallback), got {t.device}")
     if t.dtype != dtype:
         raise MoeError(-2, f"{name} must be {dtype}, got {t.dtype}")
     if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
         raise MoeError(-2, f"{name} must be [{rows}, {cols}], got {list(t.shape)}")
-    if t.is_contiguous():
-        return cols
     if cols > 1 and t.stride(1) != 1:
         raise MoeError(-2, f"{name}: the elements of a row must be contiguous")
     if rows <= 1:
@@ -265,23 +278,24 @@ def _rows(t, name, rows, cols, dtype, like):
     return t.stride(0)
 
 
-def _vector(t, name, n, dtype, like):
-    if t.device != like.device:
-        raise MoeError(-1, f"{name} must be on {like.device} (no CPU fallback), got {t.device}")
+def _vector(t, name, n, dtype, dev):
+    if t.device != dev:
+        raise MoeError(-1, f"{name} must be on {dev} (no CPU fallback), got {t.device}")
     if t.dtype != dtype:
         raise MoeError(-2, f"{name} must be {dtype}, got {t.dtype}")
     if t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
         raise MoeError(-2, f"{name} must be a contiguous [{n}], got {list(t.shape)}")
 
 
-def _call_on(device, fn, *args):
-    """fn(*args, stream) with `device` current: a kernel goes to its tensors' device, on
-    that device's current stream."""
-    torch = _torch()
-    if device.index == torch.cuda.current_device():
-        return fn(*args, torch.cuda.current_stream(device).cuda_stream)
-    with torch.cuda.device(device):
-        return fn(*args, torch.cuda.current_stream(device).cuda_stream)
+def _call_on(dev, fn, *args):
+    """fn(*args, stream) with `dev` current: a kernel goes to its tensors' device, on that
+    device's current stream."""
+    c = _cu()
+    index = dev.index
+    if index == c.current_device():
+        return fn(*args, c.stream(index))
+    with c.device(index):
+        return fn(*args, c.stream(index))
 
 
 def moe_router_select(logits, topK: int = 2, bias=None, numGroups: int = 1, topGroups: int = 1, groupTop: int = 1,
@@ -294,32 +308,35 @@ def moe_router_select(logits, topK: int = 2, bias=None, numGroups: int = 1, topG
     (a group is worth its largest key, or its two largest with groupTop=2); weights are
     renormalised over the K chosen and scaled on request.  `weights` may be a preallocated
     fp16 or fp32 tensor.  Rows of `logits` may be padded (any row stride)."""
-    torch = _torch()
-    if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
+    c = _cu()
+    if not isinstance(logits, c.Tensor) or not logits.is_cuda:
         raise MoeError(-1, "logits must be a CUDA tensor (no CPU fallback)")
-    lt = _dtype_codes().get(logits.dtype)
+    lt = c.codes.get(logits.dtype)
     if lt is None or logits.dim() != 2:
         raise MoeError(-2, "logits must be a [T, E] matrix of float32, float16 or bfloat16")
-    if scoreFunc not in SCORE_FUNCS:
+    score = SCORE_FUNCS.get(scoreFunc)
+    if score is None:
         raise MoeError(-5, f"scoreFunc {scoreFunc!r}")
     T, E = logits.shape
     K = topK if topK > 0 else 2
-    ldl = _rows(logits, "logits", T, E, logits.dtype, logits)
+    dev = logits.device
+    ldl = _rows(logits, "logits", T, E, logits.dtype, dev)
     if bias is not None:
-        _vector(bias, "bias", E, torch.float32, logits)
+        _vector(bias, "bias", E, c.f32, dev)
     if expert_ids is None:
-        expert_ids = torch.empty((T, K), dtype=torch.int32, device=logits.device)
-    elif _rows(expert_ids, "expert_ids", T, K, torch.int32, logits) != K:
+        expert_ids = c.empty((T, K), dtype=c.i32, device=dev)
+    elif _rows(expert_ids, "expert_ids", T, K, c.i32, dev) != K:
         raise MoeError(-2, "expert_ids must be contiguous")
+    wt = 1
     if weights is None:
-        weights = torch.empty((T, K), dtype=torch.float16, device=logits.device)
-    elif _rows(weights, "weights", T, K, torch.float32 if weights.dtype == torch.float32 else torch.float16,
-               logits) != K:
-        raise MoeError(-2, "weights must be contiguous")
-    _check(_call_on(logits.device, lib().MoeRouterSelect, logits.data_ptr(), lt, ldl,
-                    None if bias is None else bias.data_ptr(), expert_ids.data_ptr(), weights.data_ptr(),
-                    0 if weights.dtype == torch.float32 else 1, T, E, K, numGroups, topGroups, groupTop,
-                    SCORE_FUNCS[scoreFunc], renormalize, scale), "MoeRouterSelect")
+        weights = c.empty((T, K), dtype=c.f16, device=dev)
+    else:
+        wt = 0 if weights.dtype is c.f32 else 1
+        if _rows(weights, "weights", T, K, c.f16 if wt else c.f32, dev) != K:
+            raise MoeError(-2, "weights must be contiguous")
+    _check(_call_on(dev, lib().MoeRouterSelect, logits.data_ptr(), lt, ldl, None if bias is None else bias.data_ptr(),
+                    expert_ids.data_ptr(), weights.data_ptr(), wt, T, E, K, numGroups, topGroups, groupTop, score,
+                    renormalize, scale), "MoeRouterSelect")
     return expert_ids, weights
 
 
@@ -331,39 +348,40 @@ def moe_linear(x, weight, bias=None, activation: str = "none", gated: bool = Fal
     y = act(gate) * up + residual.  y has x's dtype, or float32 (out_dtype, or the dtype of
     a given y); residual has y's dtype and may be y itself.  Rows of every matrix may be
     padded; K and the row strides of x and weight are multiples of 8."""
-    torch = _torch()
-    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+    c = _cu()
+    if not isinstance(x, c.Tensor) or not x.is_cuda:
         raise MoeError(-1, "x must be a CUDA tensor (no CPU fallback)")
-    codes = _dtype_codes()
+    codes = c.codes
     dt = x.dtype
-    if dt not in codes or dt == torch.float32 or x.dim() != 2:
+    if dt not in codes or dt is c.f32 or x.dim() != 2:
         raise MoeError(-2, "x must be a [T, K] matrix of float16 or bfloat16")
-    if activation not in ACTIVATIONS:
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         raise MoeError(-5, f"activation {activation!r}")
     if weight.dim() != 2 or (gated and weight.shape[0] & 1):
         raise MoeError(-2, "weight must be [N, K], or [2N, K] when gated")
     T, K = x.shape
     rows = weight.shape[0]
     N = rows // 2 if gated else rows
-    ldx = _rows(x, "x", T, K, dt, x)
-    ldw = _rows(weight, "weight", rows, K, dt, x)
+    dev = x.device
+    ldx = _rows(x, "x", T, K, dt, dev)
+    ldw = _rows(weight, "weight", rows, K, dt, dev)
     if bias is not None:
-        _vector(bias, "bias", rows, dt, x)
+        _vector(bias, "bias", rows, dt, dev)
     if y is None:
         ot = out_dtype if out_dtype is not None else (residual.dtype if residual is not None else dt)
-        y = torch.empty((T, N), dtype=ot, device=x.device)
+        y = c.empty((T, N), dtype=ot, device=dev)
     else:
         ot = y.dtype
         if out_dtype is not None and out_dtype != ot:
             raise MoeError(-2, f"y must be {out_dtype}, got {ot}")
     if ot not in codes:
         raise MoeError(-5, f"y of {ot}")
-    ldy = _rows(y, "y", T, N, ot, x)
-    ldr = _rows(residual, "residual", T, N, ot, x) if residual is not None else 0
-    _check(_call_on(x.device, lib().MoeLinear, x.data_ptr(), weight.data_ptr(),
-                    None if bias is None else bias.data_ptr(), None if residual is None else residual.data_ptr(),
-                    y.data_ptr(), T, K, N, ldx, ldw, ldr, ldy, codes[dt], codes[ot], ACTIVATIONS[activation],
-                    gated), "MoeLinear")
+    ldy = _rows(y, "y", T, N, ot, dev)
+    ldr = _rows(residual, "residual", T, N, ot, dev) if residual is not None else 0
+    _check(_call_on(dev, lib().MoeLinear, x.data_ptr(), weight.data_ptr(), None if bias is None else bias.data_ptr(),
+                    None if residual is None else residual.data_ptr(), y.data_ptr(), T, K, N, ldx, ldw, ldr, ldy,
+                    codes[dt], codes[ot], act, gated), "MoeLinear")
     return y
 
 
@@ -411,7 +429,7 @@ def moe_shared_layer_forward(x, w_router, expert_weights, shared_gate_up=None, s
         if tuple(expert_ids.shape) != (T, K) or expert_ids.device != x.device:
             raise MoeError(-2, f"expert_ids must be [{T}, {K}] on {x.device}")
     if router_bias is not None:
-        _vector(router_bias, "router_bias", E, torch.float32, x)
+        _vector(router_bias, "router_bias", E, torch.float32, x.device)
     if y is None:
         y = torch.empty((T, H), dtype=f16, device=x.device)
     if workspace is None:
