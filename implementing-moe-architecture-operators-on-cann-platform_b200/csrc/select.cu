@@ -39,13 +39,9 @@ __device__ __forceinline__ bool sel_open(float v) { return v > -CUDART_INF_F; }
 
 __device__ __forceinline__ float warp_max(float v)
 {
-    for (int d = 16; d; d >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
-    return v;
-}
-__device__ __forceinline__ float warp_sum(float v)
-{
-    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-    return v;
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
 }
 
 struct ExactScratch {
@@ -53,57 +49,86 @@ struct ExactScratch {
     double group[SEL_MAX_G];
 };
 
-// The K chosen experts of one token, by one warp, with keys in 64 bits.  Lane r < K
-// gets slot r's expert; `closed` tells whether that slot had no open expert left.
-template <typename LT>
-__device__ __noinline__ int select_exact(const SelectArgs& a, const LT* row, ExactScratch& s, bool& closed)
+// Doubles as unsigned integers in the same order, none of them 0 (NaN does not occur).
+__device__ __forceinline__ unsigned long long sel_ordered(double v)
 {
+    const long long b = __double_as_longlong(v + 0.0);  // one zero of two
+    return (unsigned long long)(b ^ ((b >> 63) | (long long)0x8000000000000000ull));
+}
+
+// Called, not inlined: fetched once per call site, the code took longer than it runs.
+__device__ __noinline__ double sel_sigmoid64(float l) { return 1.0 / (1.0 + exp(-(double)l)); }
+__device__ __noinline__ double sel_exp64(float l, float mx) { return l == mx ? 1.0 : exp((double)l - (double)mx); }
+
+// The K chosen experts of one token, by one warp, with keys in 64 bits.  Returns to lane
+// r < K slot r's expert, plus 256 where no open expert was left for that slot.
+template <typename LT>
+__device__ __noinline__ int select_exact(const SelectArgs& a, const LT* row, ExactScratch& s)
+{
+    constexpr int N = SEL_MAX_E / 32;  // expert lane + 32 i is this lane's i-th
     const int lane = threadIdx.x & 31;
     const int E = a.E, size = a.E / a.G;
     const double NINF = -CUDART_INF;
-    // keys: the logits order like their scores, so scores are only needed where they
-    // are added to something
+    // the logits order like their scores, so scores are only needed where something is added
     const bool use_score = a.bias != nullptr || (a.G > 1 && a.groupTop > 1);
-    float mx = -CUDART_INF_F;
-    double total = 0.0;
-    if (use_score && !a.sigmoid) {
-        for (int e = lane; e < E; e += 32) {
-            const float l = sel_load(row, e);
-            if (sel_open(l)) mx = fmaxf(mx, l);
-        }
+    float l[N];
+    double key[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) l[i] = lane + 32 * i < E ? fmaxf(sel_load(row, lane + 32 * i), -CUDART_INF_F) : -CUDART_INF_F;
+    if (!use_score) {
+#pragma unroll
+        for (int i = 0; i < N; i++) key[i] = (double)l[i];
+    } else if (a.sigmoid) {
+#pragma unroll
+        for (int i = 0; i < N; i++) key[i] = sel_sigmoid64(l[i]);
+    } else {
+        float mx = -CUDART_INF_F;
+#pragma unroll
+        for (int i = 0; i < N; i++) mx = fmaxf(mx, l[i]);
         mx = warp_max(mx);
-        for (int e = lane; e < E; e += 32) {
-            const float l = sel_load(row, e);
-            if (sel_open(l)) total += l == mx ? 1.0 : exp((double)l - (double)mx);
+        double total = 0.0;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            key[i] = sel_open(l[i]) ? sel_exp64(l[i], mx) : 0.0;
+            total += key[i];
         }
         for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+#pragma unroll
+        for (int i = 0; i < N; i++) key[i] /= total;
     }
-    for (int e = lane; e < E; e += 32) {
-        const float l = sel_load(row, e);
-        double k = NINF;
-        if (sel_open(l)) {
-            k = (double)l;
-            if (use_score) {
-                k = a.sigmoid ? 1.0 / (1.0 + exp(-(double)l)) : (l == mx ? 1.0 : exp((double)l - (double)mx)) / total;
-                if (a.bias) {
-                    const float b = a.bias[e];
-                    k = sel_open(b) ? k + (double)b : NINF;
-                }
-            }
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        bool open = sel_open(l[i]);
+        if (a.bias && open) {
+            const float b = a.bias[lane + 32 * i];
+            open = sel_open(b);
+            key[i] += (double)b;
         }
-        s.key[e] = k;
+        if (!open) key[i] = NINF;
     }
-    __syncwarp();
     if (a.G > 1) {
-        if (lane < a.G) {
-            double m1 = NINF, m2 = NINF;
-            for (int i = 0; i < size; i++) {
-                const double k = s.key[lane * size + i];
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if (lane + 32 * i < E) s.key[lane + 32 * i] = key[i];
+        __syncwarp();
+        // the two largest keys of each group, by 32 / G' lanes (G' the next power of two)
+        int shift = 5;
+        while ((a.G - 1) >> (5 - shift)) shift--;
+        const int grp = lane >> shift;
+        double m1 = NINF, m2 = NINF;
+        if (grp < a.G)
+            for (int i = lane & ((1 << shift) - 1); i < size; i += 1 << shift) {
+                const double k = s.key[grp * size + i];
                 m2 = fmax(m2, fmin(m1, k));
                 m1 = fmax(m1, k);
             }
-            s.group[lane] = (a.groupTop > 1 && m2 > NINF) ? m1 + m2 : m1;
+        for (int d = (1 << shift) >> 1; d; d >>= 1) {
+            const double o1 = __shfl_xor_sync(0xffffffffu, m1, d), o2 = __shfl_xor_sync(0xffffffffu, m2, d);
+            m2 = fmax(fmin(m1, o1), fmax(m2, o2));
+            m1 = fmax(m1, o1);
         }
+        if (grp < a.G) s.group[grp] = (a.groupTop > 1 && m2 > NINF) ? m1 + m2 : m1;
         __syncwarp();
         bool drop = false;
         if (lane < a.G) {
@@ -113,64 +138,68 @@ __device__ __noinline__ int select_exact(const SelectArgs& a, const LT* row, Exa
             drop = before >= a.topG;
         }
         const unsigned dropped = __ballot_sync(0xffffffffu, drop);
-        for (int e = lane; e < E; e += 32)
-            if ((dropped >> (e / size)) & 1u) s.key[e] = NINF;
-        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if (lane + 32 * i < E && ((dropped >> ((lane + 32 * i) / size)) & 1u)) key[i] = NINF;
     }
-    // K times the largest key, lowest id first; a taken expert's key becomes NaN
+    // K times the largest key, lowest id first; a taken expert, or one that does not exist,
+    // is 0
+    unsigned long long u[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) u[i] = lane + 32 * i < E ? sel_ordered(key[i]) : 0ull;
+    const unsigned long long shut = sel_ordered(NINF);
     int mine = 0;
-    closed = false;
     for (int r = 0; r < a.K; r++) {
-        double best = NINF;
-        int at = SEL_MAX_E;
-        for (int e = lane; e < E; e += 32) {
-            const double k = s.key[e];
-            if (k > best || (k == best && e < at)) {
-                best = k;
-                at = e;
+        unsigned long long best = u[0];
+        int at = lane;
+#pragma unroll
+        for (int i = 1; i < N; i++)
+            if (u[i] > best) {
+                best = u[i];
+                at = lane + 32 * i;
             }
-        }
-        for (int d = 16; d; d >>= 1) {
-            const double ob = __shfl_xor_sync(0xffffffffu, best, d);
-            const int oa = __shfl_xor_sync(0xffffffffu, at, d);
-            if (ob > best || (ob == best && oa < at)) {
-                best = ob;
-                at = oa;
-            }
-        }
-        if (lane == r) {
-            mine = at;
-            closed = best == NINF;
-        }
-        if (lane == (at & 31)) s.key[at] = CUDART_NAN;
-        __syncwarp();
+        const unsigned hi = __reduce_max_sync(0xffffffffu, (unsigned)(best >> 32));
+        const bool in = (unsigned)(best >> 32) == hi;
+        const unsigned lo = __reduce_max_sync(0xffffffffu, in ? (unsigned)best : 0u);
+        const unsigned long long top = (unsigned long long)hi << 32 | lo;
+        const int e = (int)__reduce_min_sync(0xffffffffu, best == top ? (unsigned)at : 0xffffu);
+        if (lane == r) mine = e + (top == shut ? SEL_MAX_E : 0);
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if (e == lane + 32 * i) u[i] = 0ull;
     }
     return mine;
 }
 
 // ---------------------------------------------------------------------- fast path
-// LPT lanes per token (8: four tokens to a warp, 32: one).  Group g belongs to L = LPT / G'
-// lanes, G' the next power of two; each holds up to C consecutive experts of it.  A key is
-// one fp32 number whose lowest 8 bits give way to 255 - e, so that sorting and comparing move
-// one register per expert.  What that rounding, or the fast exp and quotient, may have turned
-// around is noticed: neighbours among the K + 1 best, or a group that stays and one that does
-// not, closer than the bounds below send the token to select_exact.  About one token in a
-// hundred goes there, and so do those with too few open experts.
-// Closed experts have the key -inf; open ones a finite one (+-SEL_MAX at most).
+// LPT lanes per token (8: four tokens to a warp, 32: one).  Group g belongs to LPT / G' lanes,
+// G' the next power of two; each holds consecutive experts of it.  A key is one fp32 number
+// whose lowest 8 bits give way to 255 - e, so that sorting and comparing move one register
+// per expert; eight keys at a time are sorted by a network and merged into the lane's eight
+// largest, and the lanes' lists into the token's.
+//
+// A sigmoid's keys are taken less 1 where the token's largest logit is positive: the best
+// scores are close to 1, and what is left of them is smaller and so finer in its 24 bits.
+//
+// What the lost bits or the fast exp and quotient may have turned around is noticed.
+// Neighbours among the K + 1 best closer than the bounds below are compared once more by the
+// difference of their keys (sel_before), which fp32 knows to a few millionths of itself.
+// Groups too close, a closed expert among those that count, or differences that cancel send
+// the token to a list, which select_slow settles in 64 bits when the warp is through.
 constexpr float SEL_MAX = 3.4028235e38f;
+constexpr float SEL_CLOSED = -3.4e38f;  // keys at or below: closed, or as low as can be
 #define SEL_NINF (-CUDART_INF_F)
 
 template <int LPT>
 __device__ __forceinline__ float sub_max(float v)
 {
     if constexpr (LPT == 32) {
-        float r;
-        asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-        return r;
-    }
+        return warp_max(v);
+    } else {
 #pragma unroll
-    for (int d = LPT / 2; d; d >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
-    return v;
+        for (int d = LPT / 2; d; d >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+        return v;
+    }
 }
 template <int LPT>
 __device__ __forceinline__ float sub_sum(float v)
@@ -214,6 +243,21 @@ __device__ __forceinline__ void sel_merge8(float* a, const float* b)
             if (!(i & d)) sel_order(a[i], a[i + d]);
 }
 
+// exp2 and 1 / x by the special function unit, what is below fp32's normal range as 0
+__device__ __forceinline__ float sel_ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float sel_rcp(float x)
+{
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+constexpr float SEL_LOG2E = 1.4426950408889634f;
+
 // The weight of this lane's slot (lanes whose slot does not exist or is closed return 0).
 // mx, total: softmax maximum and sum over the row (used without renormalisation only).
 //   renormalised softmax: e^(l - m) / sum, m the largest chosen logit
@@ -242,255 +286,446 @@ __device__ __forceinline__ float sel_weight(const SelectArgs& a, float l, bool o
     return w * a.scale;
 }
 
-// Position of expert e in a staged row: 4 floats of padding after every 32, so that lanes
-// that read 16 bytes at strides of 4, 8, 16 or 32 floats meet different banks.
-__device__ __forceinline__ int sel_at(int e) { return e + ((e >> 5) << 2); }
-constexpr int SEL_ROW = SEL_MAX_E + SEL_MAX_E / 32 * 4;
-
-// A row of logits into shared memory as floats, NaN as -inf, by the LPT lanes of a token.
-template <int LPT, typename LT>
-__device__ __forceinline__ void sel_stage(const LT* row, float* dst, int E, int sub, bool vec)
+// Staged rows keep their type.  WHOLE (every lane has the same number of experts, a multiple
+// of 8): 16 bytes of padding follow every 128, so that lanes that read 16 bytes at strides of
+// 16 to 128 bytes meet different banks.
+template <bool WHOLE>
+__device__ __forceinline__ int sel_at(int byte)
 {
-    constexpr int V = 16 / (int)sizeof(LT);
-    if (vec) {
-        constexpr int MAXV = SEL_MAX_E / V / LPT;  // 16-byte pieces per lane
-        uint4 q[MAXV];
+    return WHOLE ? byte + ((byte >> 7) << 4) : byte;
+}
+constexpr int SEL_ROW = SEL_MAX_E * 4 + SEL_MAX_E * 4 / 128 * 16;  // bytes, of floats
+
+template <bool WHOLE, typename LT>
+__device__ __forceinline__ float sel_get(const uint8_t* row, int e)
+{
+    return sel_load(reinterpret_cast<const LT*>(row + sel_at<WHOLE>(e * (int)sizeof(LT))), 0);
+}
+
+// Eight experts of a staged row from `first` on, `pad` where i >= n.
+template <bool WHOLE, typename LT>
+__device__ __forceinline__ void sel_chunk(float (&v)[8], const uint8_t* row, int first, int n, float pad)
+{
+    if constexpr (WHOLE) {
+        uint4 q[sizeof(LT) / 2];
+        const uint8_t* src = row + sel_at<true>(first * (int)sizeof(LT));  // (32 bytes never straddle a padding)
 #pragma unroll
-        for (int i = 0; i < MAXV; i++) {
-            const int e = (i * LPT + sub) * V;
-            if (e < E) q[i] = *reinterpret_cast<const uint4*>(row + e);
-        }
+        for (int i = 0; i < (int)sizeof(LT) / 2; i++) q[i] = *reinterpret_cast<const uint4*>(src + 16 * i);
 #pragma unroll
-        for (int i = 0; i < MAXV; i++) {
-            const int e = (i * LPT + sub) * V;
-            if (e < E) {
-                const LT* x = reinterpret_cast<const LT*>(&q[i]);
-#pragma unroll
-                for (int j = 0; j < V; j += 4)
-                    *reinterpret_cast<float4*>(dst + sel_at(e + j)) =
-                        make_float4(fmaxf(sel_load(x, j), -CUDART_INF_F), fmaxf(sel_load(x, j + 1), -CUDART_INF_F),
-                                    fmaxf(sel_load(x, j + 2), -CUDART_INF_F), fmaxf(sel_load(x, j + 3), -CUDART_INF_F));
-            }
-        }
+        for (int i = 0; i < 8; i++) v[i] = sel_load(reinterpret_cast<const LT*>(q), i);
     } else {
-#pragma unroll 8
-        for (int e = sub; e < E; e += LPT) dst[sel_at(e)] = fmaxf(sel_load(row, e), -CUDART_INF_F);
+        const LT* src = reinterpret_cast<const LT*>(row) + first;
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = i < n ? sel_load(src, i) : pad;
     }
 }
 
-struct SelectPlan {
-    int lanes_shift;  // log2 of the lanes per group
-    int per_lane;     // experts per lane, at most C
-    bool whole;       // per_lane == C everywhere: 16-byte reads of the staged row
-    bool vec;         // rows of logits start on 16-byte boundaries and hold whole 16 bytes
-    bool by_logit;    // no bias and no sums of scores: the logits order as their scores do
+// Starts the copy of a row of logits into shared memory, by the LPT lanes of a token;
+// asynchronously, where 16 (vec) or 4 bytes can be.
+template <int LPT, bool WHOLE, typename LT>
+__device__ __forceinline__ void sel_stage(const LT* row, uint8_t* dst, int E, int sub, bool vec)
+{
+    const uint32_t d = smem_u32(dst);
+    const uint8_t* src = reinterpret_cast<const uint8_t*>(row);
+    const int bytes = E * (int)sizeof(LT);
+    if (vec) {
+        for (int o = sub * 16; o < bytes; o += LPT * 16)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d + sel_at<WHOLE>(o)), "l"(src + o) : "memory");
+    } else if (sizeof(LT) == 4) {
+        for (int o = sub * 4; o < bytes; o += LPT * 4)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(d + sel_at<WHOLE>(o)), "l"(src + o) : "memory");
+    } else {
+#pragma unroll 8
+        for (int e = sub; e < E; e += LPT) *reinterpret_cast<LT*>(dst + sel_at<WHOLE>(e * (int)sizeof(LT))) = row[e];
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+}
+
+__device__ __forceinline__ void sel_store(const SelectArgs& a, int t, int k, int e, float w)
+{
+    const size_t o = (size_t)t * a.K + k;
+    a.ids[o] = e;
+    if (a.wtype == MOE_DT_FLOAT)
+        static_cast<float*>(a.weights)[o] = w;
+    else
+        static_cast<__half*>(a.weights)[o] = __float2half_rn(w);
+}
+
+// Settles a listed token in 64 bits, by the whole warp.
+template <typename LT>
+__device__ __noinline__ void select_slow(const SelectArgs& a, int t, ExactScratch& scratch)
+{
+    const int lane = threadIdx.x & 31;
+    const LT* row = static_cast<const LT*>(a.logits) + (size_t)t * a.ldl;
+    float mx = SEL_NINF, total = 0.0f;
+    if (!a.sigmoid && !a.renorm) {
+        for (int e = lane; e < a.E; e += 32) mx = fmaxf(mx, sel_load(row, e));
+        mx = warp_max(mx);
+        for (int e = lane; e < a.E; e += 32) {
+            const float l = sel_load(row, e);
+            if (sel_open(l)) total += l == mx ? 1.0f : expf(l - mx);
+        }
+        total = sub_sum<32>(total);
+    }
+    const int got = select_exact<LT>(a, row, scratch);
+    const bool open = lane < a.K && got < SEL_MAX_E;
+    const int e = got & (SEL_MAX_E - 1);
+    const float w = sel_weight<32>(a, open ? sel_load(row, e) : 0.0f, open, mx, total);
+    if (lane < a.K) sel_store(a, t, lane, e, w);
+    __syncwarp();
+}
+
+// One of the K + 1 best of a token.
+struct SelBest {
+    float l, b;
+    int e;
 };
 
-template <typename LT, int LPT, int C>
-__global__ void __launch_bounds__(SEL_WARPS * 32, C == 32 ? 4 : 6) select_kernel(const SelectArgs a, const SelectPlan p)
+// Whether x comes before y, by the difference of their keys:
+//   logits   l_x - l_y;
+//   sigmoid  s_x - s_y = s_x (1 - s_y) (1 - e^-(l_x - l_y));
+//   softmax  s_x - s_y = s_y (e^(l_x - l_y) - 1);
+// plus b_x - b_y.  The first part is known to c of itself (the errors of two scores, as
+// bounded in the kernel, and of expm1), the second to 2^-24.  `lost` is set where that does
+// not decide.
+__device__ __forceinline__ bool sel_before(const SelectArgs& a, bool by_logit, const SelBest& x, const SelBest& y, float mx,
+                                           float inv, bool& lost)
 {
-    constexpr int TPW = 32 / LPT;  // tokens per warp
-    constexpr int KEEP = C < 8 ? C : 8;
+    const bool id = x.e < y.e;
+    if (by_logit) return x.l > y.l || (x.l == y.l && id);
+    if (x.l == y.l && x.b == y.b) return id;
+    const float d = x.l - y.l;
+    float A = 0.0f, c = 0.0f;
+    if (d != 0.0f) {
+        if (a.sigmoid) {
+            A = -expm1f(-d) * sel_rcp(1.0f + sel_ex2(x.l * -SEL_LOG2E)) * sel_rcp(1.0f + sel_ex2(y.l * SEL_LOG2E));
+            c = fmaxf(fabsf(x.l), fabsf(y.l)) * 4e-7f + 3e-6f;
+        } else {
+            A = expm1f(d) * sel_ex2((y.l - mx) * SEL_LOG2E) * inv;
+            c = (mx - y.l) * 2.5e-7f + 3e-6f;
+        }
+    }
+    const float B = x.b - y.b, D = A + B;
+    lost |= !(fabsf(D) > fabsf(A) * c + fabsf(B) * 2.4e-7f + 1e-36f);
+    return D > 0.0f;
+}
+
+struct SelectPlan {
+    int shift;      // log2 of the lanes per group
+    int per_lane;   // experts per lane, in chunks of 8
+    bool vec;       // rows of logits start on 16-byte boundaries and hold whole 16 bytes
+    bool by_logit;  // no bias and no sums of scores: the logits order as their scores do
+};
+
+constexpr int SEL_LIST = 32;
+
+template <typename LT, int LPT, bool WHOLE>
+__global__ void __launch_bounds__(SEL_WARPS * 32, 5) select_kernel(const SelectArgs a, const SelectPlan p)
+{
+    constexpr int TPW = 32 / LPT;              // tokens per warp
     constexpr bool EXACT16 = sizeof(LT) == 2;  // a 16-bit logit is whole in the upper 24 bits
-    __shared__ __align__(16) float rows[SEL_WARPS][TPW][SEL_ROW];
-    __shared__ __align__(16) float sbias[SEL_ROW];
-    __shared__ ExactScratch scratch[SEL_WARPS];
+    constexpr unsigned MASK = LPT == 32 ? 0xffffffffu : (1u << (LPT & 31)) - 1u;
+    constexpr int BUFS = LPT == 8 ? 2 : 1;     // (32 lanes: few tokens, hardly a second one per warp)
+    __shared__ __align__(16) uint8_t rows[SEL_WARPS][BUFS][TPW][SEL_ROW / 4 * sizeof(LT)];
+    __shared__ __align__(16) uint8_t sbias[SEL_ROW];
+    __shared__ ExactScratch scratch[LPT == 8 ? 1 : SEL_WARPS];  // (8: in the row buffer that is free then)
+    static_assert(LPT != 8 || sizeof(rows[0][0]) >= sizeof(ExactScratch), "scratch fits");
+    __shared__ int slow[SEL_WARPS][SEL_LIST];  // tokens for select_slow
     pdl_trigger();
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int sub = lane & (LPT - 1), tok = lane / LPT;
+    const int sub = lane & (LPT - 1), tok = lane / LPT, shift = tok * (LPT & 31);
     if (a.bias) {
-        for (int e = threadIdx.x; e < a.E; e += SEL_WARPS * 32) sbias[sel_at(e)] = fmaxf(a.bias[e], -CUDART_INF_F);
+        for (int e = threadIdx.x; e < a.E; e += SEL_WARPS * 32)
+            *reinterpret_cast<float*>(sbias + sel_at<WHOLE>(e * 4)) = fminf(fmaxf(a.bias[e], -SEL_MAX), SEL_MAX);
         __syncthreads();
     }
     const int size = a.E / a.G;
-    const int grp = sub >> p.lanes_shift;
-    const int first = grp * size + (sub & ((1 << p.lanes_shift) - 1)) * p.per_lane;
+    const int grp = sub >> p.shift;
+    const int first = grp * size + (sub & ((1 << p.shift) - 1)) * p.per_lane;
     const int mine = grp < a.G ? max(0, min(p.per_lane, (grp + 1) * size - first)) : 0;
-    const int step = gridDim.x * SEL_WARPS * TPW;
-    float* const row = rows[warp][tok];
-    for (int t0 = (blockIdx.x * SEL_WARPS + warp) * TPW; t0 < a.T; t0 += step) {
-        const int t = min(t0 + tok, a.T - 1);  // the last warp's spare tokens repeat the last one
-        const LT* src = static_cast<const LT*>(a.logits) + (size_t)t * a.ldl;
-        sel_stage<LPT, LT>(src, row, a.E, sub, p.vec);
-        __syncwarp();
-        // ---- keys
-        float v[C];
-        if (p.whole) {
+    const uint32_t step = gridDim.x * SEL_WARPS * TPW, T = (uint32_t)a.T;  // (T + step < 2^32)
+    // the sum of a softmax: for its scores, or for weights that are not renormalised
+    const bool soft = !a.sigmoid && !(p.by_logit && a.renorm);
+    const bool exact = EXACT16 && p.by_logit;
+    const LT* const logits = static_cast<const LT*>(a.logits);
+    auto token = [&](uint32_t from) { return (int)min(from + tok, T - 1); };  // spare tokens repeat the last one
+    uint32_t t0 = (blockIdx.x * SEL_WARPS + warp) * TPW;
+    int buf = 0;
+    if (BUFS > 1 && t0 < T) sel_stage<LPT, WHOLE, LT>(logits + (size_t)token(t0) * a.ldl, rows[warp][0][tok], a.E, sub, p.vec);
+    while (t0 < T) {
+        int listed = 0;
+        for (; t0 < T && listed + TPW <= SEL_LIST; t0 += step) {
+            const int t = token(t0);
+            const uint8_t* const row = rows[warp][buf][tok];
+            if (BUFS > 1) {
+                // the next tokens' rows come while these are worked on
+                buf ^= BUFS - 1;
+                sel_stage<LPT, WHOLE, LT>(logits + (size_t)token(t0 + step < T ? t0 + step : t0) * a.ldl, rows[warp][buf][tok], a.E,
+                                   sub, p.vec);
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+            } else {
+                sel_stage<LPT, WHOLE, LT>(logits + (size_t)t * a.ldl, rows[warp][0][tok], a.E, sub, p.vec);
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+            }
+            __syncwarp();
+            float mx = SEL_NINF, total = 0.0f;
+            if (soft || !p.by_logit) {
+                // (a sigmoid only asks whether it is positive, which some of them tell)
+                float v[8];
+                const int upto = soft ? p.per_lane : 8;
+#pragma unroll 1
+                for (int c = 0; c < upto; c += 8) {
+                    sel_chunk<WHOLE, LT>(v, row, first + c, mine - c, SEL_NINF);
 #pragma unroll
-            for (int i = 0; i < C; i += 4) {
-                const float4 q = *reinterpret_cast<const float4*>(row + sel_at(first + i));
-                v[i] = q.x;
-                v[i + 1] = q.y;
-                v[i + 2] = q.z;
-                v[i + 3] = q.w;
+                    for (int i = 0; i < 8; i++) mx = fmaxf(mx, v[i]);
+                }
+                mx = sub_max<LPT>(mx);
             }
-        } else {
+            if (soft) {
+                float v[8];
+#pragma unroll 1
+                for (int c = 0; c < p.per_lane; c += 8) {
+                    sel_chunk<WHOLE, LT>(v, row, first + c, mine - c, SEL_NINF);
+                    // (the largest apart: +inf - +inf has no difference; NaN counts as -inf)
 #pragma unroll
-            for (int i = 0; i < C; i++) v[i] = i < mine ? row[sel_at(first + i)] : -CUDART_INF_F;
-        }
-        float mx = -CUDART_INF_F, total = 0.0f;
-        if (!a.sigmoid && !(p.by_logit && a.renorm)) {
+                    for (int i = 0; i < 8; i++)
+                        total += v[i] == mx ? 1.0f : fmaxf(sel_ex2((v[i] - mx) * SEL_LOG2E), 0.0f);
+                }
+                total = sub_sum<LPT>(total);
+            }
+            const float inv = soft ? sel_rcp(total) : 1.0f;
+            const float sign = mx > 0.0f ? 1.0f : -1.0f;  // a sigmoid's keys: s - 1 or s
+            // ---- keys, eight at a time, merged into this lane's eight largest
+            float v8[8];
+#pragma unroll 1
+            for (int c = 0; c < p.per_lane; c += 8) {
+                float v[8];
+                sel_chunk<WHOLE, LT>(v, row, first + c, mine - c, SEL_NINF);
+                const int id = 255 - (first + c);
+                if (p.by_logit) {
 #pragma unroll
-            for (int i = 0; i < C; i++) mx = fmaxf(mx, v[i]);
-            mx = sub_max<LPT>(mx);
+                    for (int i = 0; i < 8; i++) {
+                        // the lower id ahead: more in the low bits of a positive number is
+                        // more, of a negative one less; + 0 makes one zero of two
+                        const int b = __float_as_int(fminf(fmaxf(v[i] + 0.0f, -SEL_MAX), SEL_MAX));
+                        v[i] = __int_as_float((b & ~255) | (((b >> 31) ^ (id - i)) & 255));
+                    }
+                } else {
+                    if (a.sigmoid) {
 #pragma unroll
-            for (int i = 0; i < C; i++) {
-                // -inf: 0 (also where the whole row is -inf); +inf: 1
-                total += v[i] > SEL_NINF ? (v[i] == mx ? 1.0f : __expf(v[i] - mx)) : 0.0f;
-            }
-            total = sub_sum<LPT>(total);
-        }
-        if (p.by_logit) {
+                        for (int i = 0; i < 8; i++) v[i] = -sign * sel_rcp(1.0f + sel_ex2(v[i] * (sign * SEL_LOG2E)));
+                    } else {
 #pragma unroll
-            for (int i = 0; i < C; i++) {
-                // the lower id ahead: more in the low bits of a positive number is more, of
-                // a negative one less; + 0 makes one zero of two
-                const int b = __float_as_int(fminf(fmaxf(v[i] + 0.0f, -SEL_MAX), SEL_MAX));
-                const float k = __int_as_float((b & ~255) | (((b >> 31) ^ (255 - (first + i))) & 255));
-                v[i] = v[i] > SEL_NINF ? k : SEL_NINF;
-            }
-        } else {
-            const float inv = __fdividef(1.0f, total);
+                        for (int i = 0; i < 8; i++) v[i] = (v[i] == mx ? 1.0f : sel_ex2((v[i] - mx) * SEL_LOG2E)) * inv;
+                    }
+                    if (a.bias) {
+                        float b[8];
+                        sel_chunk<WHOLE, float>(b, sbias, first + c, mine - c, 0.0f);
 #pragma unroll
-            for (int i = 0; i < C; i++) {
-                const float l = v[i];
-                float s = a.sigmoid ? __fdividef(1.0f, 1.0f + __expf(-l)) : (l == mx ? 1.0f : __expf(l - mx)) * inv;
-                if (a.bias) s += i < mine ? sbias[sel_at(first + i)] : 0.0f;
-                const int b = __float_as_int(fminf(fmaxf(s, -SEL_MAX), SEL_MAX));
-                const float k = __int_as_float((b & ~255) | (255 - (first + i)));
-                v[i] = l > SEL_NINF && s > SEL_NINF ? k : SEL_NINF;
-            }
-        }
-        // ---- this lane's largest, in order
-        if constexpr (C <= 8) {
-            sel_sort<C>(v);
-        } else {
-            sel_sort<8>(v);
+                        for (int i = 0; i < 8; i++) v[i] += b[i];
+                    }
 #pragma unroll
-            for (int i = 8; i < C; i += 8) {
-                sel_sort<8>(v + i);
-                sel_merge8(v, v + i);
-            }
-        }
-        bool unsure = false;
-        // ---- groups
-        if (a.G > 1) {
-            float m1 = v[0], m2 = KEEP > 1 ? v[KEEP > 1 ? 1 : 0] : SEL_NINF;
-            for (int d = (1 << p.lanes_shift) >> 1; d; d >>= 1) {
-                const float o1 = __shfl_xor_sync(0xffffffffu, m1, d), o2 = __shfl_xor_sync(0xffffffffu, m2, d);
-                m2 = fmaxf(fminf(m1, o1), fmaxf(m2, o2));
-                m1 = fmaxf(m1, o1);
-            }
-            // the low bits must not count: they are ids
-            const float k1 = __int_as_float(__float_as_int(m1) & ~255);
-            const float k2 = a.groupTop > 1 && m2 > SEL_NINF ? __int_as_float(__float_as_int(m2) & ~255) : 0.0f;
-            const float val = m1 > SEL_NINF ? fmaxf(k1 + k2, -SEL_MAX) : SEL_NINF;
-            int before = 0;
-            for (int d = 1 << p.lanes_shift; d < LPT; d += 1 << p.lanes_shift) {
-                const int from = sub ^ d;
-                const float o = __shfl_xor_sync(0xffffffffu, val, d);
-                before += (o > val || (o == val && (from >> p.lanes_shift) < grp)) ? 1 : 0;
-            }
-            const bool stay = before < a.topG;
-            if (!(EXACT16 && p.by_logit)) {
-                const float in = -sub_max<LPT>(stay ? -val : SEL_NINF);  // the least that stays
-                const float out = sub_max<LPT>(stay ? SEL_NINF : val);   // the most that does not
-                // Each key is off by 2^-15 of its size (the bits given to ids) and by its
-                // score's error: 2^-15 of it, and 2e-6 at most (see below).
-                float tol;
-                if (a.bias)
-                    tol = sub_max<LPT>(val > SEL_NINF ? fabsf(k1) + fabsf(k2) : 0.0f) * 6.2e-5f + 8e-6f;
-                else
-                    tol = (fabsf(in) + fabsf(out)) * 6.6e-5f + 1e-37f;
-                unsure = out > SEL_NINF && !(in - out > tol);
-            }
-            if (!stay) {
+                    for (int i = 0; i < 8; i++)  // (NaN becomes -SEL_MAX)
+                        v[i] = __int_as_float((__float_as_int(fmaxf(v[i], -SEL_MAX)) & ~255) | ((id - i) & 255));
+                }
+                if (!WHOLE) {
 #pragma unroll
-                for (int i = 0; i < KEEP; i++) v[i] = SEL_NINF;
-            }
-        }
-        // ---- the K + 1 largest: the largest head K + 1 times
-        float win = SEL_NINF, last = SEL_NINF;
-        for (int r = 0; r <= a.K; r++) {
-            const float m = sub_max<LPT>(v[0]);
-            if (sub == r) win = m;
-            last = m;
-            if (__float_as_int(v[0]) == __float_as_int(m)) {  // (bits: -0 is not +0)
+                    for (int i = 0; i < 8; i++)
+                        if (c + i >= mine) v[i] = SEL_NINF;
+                }
+                sel_sort<8>(v);
+                if (c == 0) {
 #pragma unroll
-                for (int i = 0; i + 1 < KEEP; i++) v[i] = v[i + 1];
-                v[KEEP - 1] = SEL_NINF;
+                    for (int i = 0; i < 8; i++) v8[i] = v[i];
+                } else {
+                    sel_merge8(v8, v);
+                }
             }
-        }
-        float next = __shfl_down_sync(0xffffffffu, win, 1);
-        if (sub == a.K - 1) next = last;
-        const bool slot = sub < a.K;
-        int e = 0;
-        if (slot && win > SEL_NINF) {
-            const int b = __float_as_int(win);
-            e = p.by_logit && b < 0 ? b & 255 : 255 - (b & 255);
-            if (next > SEL_NINF && !(EXACT16 && p.by_logit)) {
-                const float k0 = __int_as_float(b & ~255), k1 = __int_as_float(__float_as_int(next) & ~255);
-                const float big = fmaxf(fabsf(k0), fabsf(k1));
+            bool dark = false;  // for select_slow
+            // ---- groups
+            if (a.G > 1) {
+                float m1 = v8[0], m2 = v8[1];
+                for (int d = (1 << p.shift) >> 1; d; d >>= 1) {
+                    const float o1 = __shfl_xor_sync(0xffffffffu, m1, d), o2 = __shfl_xor_sync(0xffffffffu, m2, d);
+                    m2 = fmaxf(fminf(m1, o1), fmaxf(m2, o2));
+                    m1 = fmaxf(m1, o1);
+                }
+                // the low bits must not count: they are ids
+                const int b1 = __float_as_int(m1), b2 = __float_as_int(m2);
+                const float k1 = __int_as_float(b1 & ~255), k2 = __int_as_float(b2 & ~255);
+                float val = SEL_NINF, mag = 0.0f;
+                if (grp < a.G) {
+                    val = a.groupTop > 1 ? fmaxf(k1 + k2, -SEL_MAX) : k1;
+                    mag = fabsf(k1) + (a.groupTop > 1 ? fabsf(k2) : 0.0f);
+                    // the group's best, or second best, is closed: its value is another
+                    const int e1 = p.by_logit && b1 < 0 ? b1 & 255 : 255 - (b1 & 255), e2 = 255 - (b2 & 255);
+                    dark = !(m1 > SEL_CLOSED && sel_open(sel_get<WHOLE, LT>(row, e1)));
+                    if (a.groupTop > 1) dark |= !(m2 > SEL_CLOSED && sel_open(sel_get<WHOLE, LT>(row, e2)));
+                }
+                int before = 0;
+                for (int d = 1 << p.shift; d < LPT; d += 1 << p.shift) {
+                    const int from = sub ^ d;
+                    const float o = __shfl_xor_sync(0xffffffffu, val, d);
+                    before += (o > val || (o == val && (from >> p.shift) < grp)) ? 1 : 0;
+                }
+                const bool stay = before < a.topG;
+                if (!exact) {
+                    const float in = -sub_max<LPT>(stay ? -val : SEL_NINF);  // the least that stays
+                    const float out = sub_max<LPT>(stay ? SEL_NINF : val);   // the most that does not
+                    // Each key is off by 2^-15 of its size (the bits given to ids) and by its
+                    // score's error: 2^-15 of it, and 2e-6 at most, a sigmoid's 5e-7 (see
+                    // below); two keys on either side.
+                    float tol;
+                    if (a.sigmoid || a.bias)
+                        tol = sub_max<LPT>(mag) * 6.2e-5f + (a.sigmoid ? 2e-6f : 8e-6f);
+                    else
+                        tol = (fabsf(in) + fabsf(out)) * 6.6e-5f + 1e-37f;
+                    dark |= out > SEL_NINF && !(in - out > tol);
+                }
+                if (!stay) {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) v8[i] = SEL_NINF;
+                }
+            }
+            // the largest of the token's keys below x (LPT = 8); a lane whose eight are all not
+            // below has lost sight of its own next
+            auto below = [&](float x) {
+                float m = SEL_NINF;
+#pragma unroll
+                for (int i = 0; i < 8; i++) m = fmaxf(m, v8[i] < x ? v8[i] : SEL_NINF);
+                dark |= p.per_lane > 8 && v8[7] > SEL_NINF && v8[7] >= x;
+                return sub_max<LPT>(m);
+            };
+            // ---- slot r's key to lane r, and the two keys after the last slot
+            float win = SEL_NINF, after1 = SEL_NINF, after2 = SEL_NINF;
+            if constexpr (LPT == 32) {
+                // the largest head, K + 2 times
+#pragma unroll 1
+                for (int r = 0; r < a.K + 2; r++) {
+                    const float m = warp_max(v8[0]);
+                    if (sub == r) win = m;
+                    after1 = after2;
+                    after2 = m;
+                    if (__float_as_int(v8[0]) == __float_as_int(m)) {  // (bits: -0 is not +0)
+#pragma unroll
+                        for (int i = 0; i < 7; i++) v8[i] = v8[i + 1];
+                        v8[7] = SEL_NINF;
+                    }
+                }
+            } else {
+                // lists merge pairwise until every lane has the token's eight largest
+                float t8[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) t8[i] = v8[i];
+#pragma unroll 1
+                for (int d = 1; d < LPT; d *= 2) {
+                    float o[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) o[i] = __shfl_xor_sync(0xffffffffu, t8[i], d);
+                    sel_merge8(t8, o);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    if (sub == i) win = t8[i];
+                    if (a.K == i) after1 = t8[i];
+                    if (a.K + 1 == i) after2 = t8[i];
+                }
+                // the ninth: the largest below the eighth
+                if (a.K == 8) after1 = below(t8[7]);
+                if (a.K == 7) after2 = below(t8[7]);
+            }
+            const bool slot = sub < a.K;
+            auto expert = [&](float key) {
+                const int b = __float_as_int(key);
+                return !(key > SEL_NINF) ? 0 : (p.by_logit && b < 0 ? b & 255 : 255 - (b & 255));
+            };
+            auto value = [&](float key) { return key > SEL_NINF ? __int_as_float(__float_as_int(key) & ~255) : SEL_NINF; };
+            int e = slot ? expert(win) : 0, at = sub;
+            float l = sel_get<WHOLE, LT>(row, e);
+            if (slot) dark |= !(win > SEL_CLOSED && sel_open(l));
+            if (!exact) {
                 // Two keys with truncated values this far apart are in order: a step of the
                 // truncation (2^-15 of the key) and twice a score's error.  A sigmoid is off
-                // by s (1 - s) (1.44 |l| + 4) 2^-23 + 2^-22 s < 4e-7, a softmax by
-                // (3 |l - m| + 31) 2^-24 s < 2e-6; relative to s, both by less than 2^-15 down
-                // to where fp32 ends.
-                if (p.by_logit)
-                    unsure |= k0 == k1;
-                else
-                    unsure |= !(k0 - k1 > (a.bias ? big * 3.08e-5f + 4e-6f : big * 9.2e-5f + 1e-37f));
+                // by s (1 - s) (1.44 |l| + 4) 2^-23 + 2^-22 min(s, 1 - s) < 5e-7, a softmax by
+                // (3 |l - m| + 31) 2^-24 s < 2e-6; relative to s, both by less than 2^-15
+                // down to where fp32 ends.  A logit is exact.
+                const float rel = a.bias || a.sigmoid ? 3.08e-5f : 9.2e-5f;
+                const float abs = a.sigmoid ? 1e-6f : (a.bias ? 4e-6f : 1e-37f);
+                auto apart = [&](float hi, float lo) {
+                    return lo == SEL_NINF || (p.by_logit ? hi != lo : hi - lo > fmaxf(fabsf(hi), fabsf(lo)) * rel + abs);
+                };
+                const float next = __shfl_down_sync(0xffffffffu, win, 1);
+                const bool doubt = slot && !apart(value(win), value(sub == a.K - 1 ? after1 : next));
+                if (__any_sync(0xffffffffu, doubt)) {
+                    // compare once more, everyone with everyone and with the one after
+                    if (LPT == 8 && a.K == 8) after2 = below(after1);
+                    if (sub == a.K - 1 && doubt) dark |= !apart(value(after1), value(after2));  // a third at the border
+                    const SelBest me = {l, a.bias ? sel_get<WHOLE, float>(sbias, e) : 0.0f, e};
+                    SelBest other;
+                    bool lost = false, beaten = false;
+                    int before = 0;
+#pragma unroll 1
+                    for (int j = 0; j <= a.K; j++) {
+                        if (j < a.K) {
+                            other.l = __shfl_sync(0xffffffffu, me.l, shift + j);
+                            other.b = __shfl_sync(0xffffffffu, me.b, shift + j);
+                            other.e = __shfl_sync(0xffffffffu, me.e, shift + j);
+                        } else {
+                            other.e = expert(after1);
+                            other.l = sel_get<WHOLE, LT>(row, other.e);
+                            other.b = a.bias ? sel_get<WHOLE, float>(sbias, other.e) : 0.0f;
+                        }
+                        beaten = false;
+                        if (j != sub && (j < a.K || after1 > SEL_NINF))
+                            beaten = sel_before(a, p.by_logit, other, me, mx, inv, lost);
+                        before += beaten ? 1 : 0;
+                    }
+                    if (slot) dark |= lost;
+                    const unsigned less = __ballot_sync(0xffffffffu, slot && beaten);  // those that the one after beats
+                    at = before;
+                    if (slot && before >= a.K) {  // it takes the place of the one that falls out
+                        e = other.e;
+                        l = other.l;
+                        at = a.K - __popc((less >> shift) & MASK);
+                        dark |= !(after1 > SEL_CLOSED && sel_open(l));
+                    }
+                }
             }
-        } else if (slot) {
-            unsure = true;  // too few open experts
-        }
-        bool closed = false;
-        // ---- tokens to be told apart exactly, by the whole warp
-        for (unsigned todo = __ballot_sync(0xffffffffu, unsure); todo;) {
-            const int which = (__ffs(todo) - 1) / LPT;
-            const int tt = __shfl_sync(0xffffffffu, t, which * LPT);
-            bool shut;
-            const int got = select_exact<LT>(a, static_cast<const LT*>(a.logits) + (size_t)tt * a.ldl, scratch[warp], shut);
-            const int ge = __shfl_sync(0xffffffffu, got, sub);
-            const bool gs = __shfl_sync(0xffffffffu, (int)shut, sub) != 0;
-            if (tok == which) {
-                e = slot ? ge : 0;
-                closed = slot && gs;
+            const float w = sel_weight<LPT>(a, l, slot, mx, total);
+            const unsigned darks = __ballot_sync(0xffffffffu, dark);
+            if (slot && t0 + tok < T && !((darks >> shift) & MASK)) sel_store(a, t, at, e, w);
+            if (darks) {
+#pragma unroll 1
+                for (int k = 0; k < TPW && t0 + k < T; k++)
+                    if ((darks >> (k * (LPT & 31))) & MASK) slow[warp][listed++] = (int)t0 + k;
             }
-            todo &= ~((LPT == 32 ? 0xffffffffu : ((1u << (LPT & 31)) - 1u)) << (which * (LPT & 31)));
-            if (LPT == 32) todo = 0;
+            __syncwarp();
         }
-        const bool open = slot && !closed;
-        const float w = sel_weight<LPT>(a, open ? row[sel_at(e)] : 0.0f, open, mx, total);
-        if (slot && t0 + tok < a.T) {
-            const size_t o = (size_t)t * a.K + sub;
-            a.ids[o] = e;
-            if (a.wtype == MOE_DT_FLOAT)
-                static_cast<float*>(a.weights)[o] = w;
-            else
-                static_cast<__half*>(a.weights)[o] = __float2half_rn(w);
-        }
+#pragma unroll 1
+        for (int i = 0; i < listed; i++)
+            select_slow<LT>(a, slow[warp][i],
+                            LPT == 8 ? *reinterpret_cast<ExactScratch*>(rows[warp][buf ^ (BUFS - 1)]) : scratch[warp]);
         __syncwarp();
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 namespace {
 
-template <typename LT, int LPT, int C>
-cudaError_t launch_select_as(const SelectArgs& a, SelectPlan p, cudaStream_t s)
+template <typename LT, int LPT>
+cudaError_t launch_select_as(const SelectArgs& a, SelectPlan p, int groups, cudaStream_t s)
 {
-    int groups = 1, shift = 0;
-    while (groups < a.G) groups *= 2;
-    while ((LPT / groups) >> (shift + 1)) shift++;
-    const int size = a.E / a.G, lanes = 1 << shift;
-    p.lanes_shift = shift;
+    const int size = a.E / a.G, lanes = LPT / groups;
+    p.shift = 0;
+    while (lanes >> (p.shift + 1)) p.shift++;
     p.per_lane = (size + lanes - 1) / lanes;
-    p.whole = a.G == groups && size == lanes * C;
+    const bool whole = a.G == groups && size == lanes * p.per_lane && p.per_lane % 8 == 0;
     constexpr int per_block = SEL_WARPS * (32 / LPT);
     const long long blocks = ((long long)a.T + per_block - 1) / per_block;
-    return launch_pdl(select_kernel<LT, LPT, C>, dim3((unsigned)(blocks < 148 * 6 ? blocks : 148 * 6)),
-                      dim3(SEL_WARPS * 32), 0, s, a, p);
+    const long long most = 148 * 5;  // as many as run at once; each then takes several sets of tokens
+    return launch_pdl(whole ? select_kernel<LT, LPT, true> : select_kernel<LT, LPT, false>,
+                      dim3((unsigned)(blocks < most ? blocks : most)), dim3(SEL_WARPS * 32), 0, s, a, p);
 }
 
 template <typename LT>
@@ -502,17 +737,8 @@ cudaError_t launch_select_type(const SelectArgs& a, cudaStream_t s)
     p.by_logit = !a.bias && (a.G == 1 || a.groupTop == 1);
     int groups = 1;
     while (groups < a.G) groups *= 2;
-    const int size = a.E / a.G;
-    if (groups <= 8 && a.T >= 1024) {
-        const int per = (size + 8 / groups - 1) / (8 / groups);
-        if (per <= 4) return launch_select_as<LT, 8, 4>(a, p, s);
-        if (per <= 8) return launch_select_as<LT, 8, 8>(a, p, s);
-        if (per <= 16) return launch_select_as<LT, 8, 16>(a, p, s);
-        if (per <= 32) return launch_select_as<LT, 8, 32>(a, p, s);
-    }
-    const int per = (size + 32 / groups - 1) / (32 / groups);
-    if (per <= 8) return launch_select_as<LT, 32, 8>(a, p, s);
-    return launch_select_as<LT, 32, 16>(a, p, s);
+    if (groups <= 8 && a.T >= 1024) return launch_select_as<LT, 8>(a, p, groups, s);
+    return launch_select_as<LT, 32>(a, p, groups, s);
 }
 
 }  // namespace
