@@ -127,6 +127,27 @@ def test_activations(moe, gpu, act, gated):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(1, 14336, 64), (8, 8192, 300), (16, 14336, 40), (100, 14336, 64), (300, 8192, 256),
+                                   (700, 14336, 1000), (4096, 4096, 64)])
+def test_fp32_sums_are_rounded(moe, gpu, shape):
+    """An fp32 y over many products: the tensor cores cut their sums off, so a sum of n
+    products of one sign is off by up to n / 16 half ulps to one side.  Segments of at most
+    512 products bound that by 32 + (their number) roundings of 2^-24: positive inputs show
+    it, where a single accumulator over K = 14336 is off by hundreds."""
+    T, K, N = shape
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = (torch.rand((T, K), generator=g, device="cuda") + 0.5).half()
+    w = (torch.rand((N, K), generator=g, device="cuda") + 0.5).half()
+    y = moe.moe_linear(x, w, out_dtype=torch.float32).double()
+    want = x.double() @ w.double().t()
+    # a k split leaves at most K / 2 to one CTA, which has 4 accumulators: segments of up to
+    # K / 8 products, each 16 of them cut off by at most 2 units of 2^-24 of the sum
+    seg = max(512, K // 8)
+    rel = (seg / 16 * 2 + K / 512 + 8) * 2.0 ** -24
+    assert ((y - want).abs() <= rel * want).all(), ((y - want) / want).abs().max().item() * 2 ** 24
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("T", [1, 9, 50, 200])
 def test_activation_range(moe, gpu, T):
     """Sums from far below to far above zero: identity weights, x over a wide range."""

@@ -73,9 +73,19 @@ def check(moe, logits, K, wtype=None, **kw):
         w0 = torch.full((logits.shape[0], K), 7.0, dtype=torch.float32, device="cuda")
     names = dict(G="numGroups", topG="topGroups", groupTop="groupTop", score="scoreFunc", renorm="renormalize",
                  scale="scale", bias="bias")
-    ids, w = moe.moe_router_select(logits, K, weights=w0, **{names[k]: v for k, v in kr.items()})
-    torch.cuda.synchronize()
+    call = {names[k]: v for k, v in kr.items()}
     rid, rw = reference(logits, K, **kw)
+    judge(*moe.moe_router_select(logits, K, weights=w0, **call), rid, rw)
+    # the same rows many times over: large batches share a warp between tokens
+    T = logits.shape[0]
+    n = -(-1100 // T)
+    many = logits.repeat(n, 1)
+    w0 = None if w0 is None else w0.repeat(n, 1)
+    judge(*moe.moe_router_select(many, K, weights=w0, **call), np.tile(rid, (n, 1)), np.tile(rw, (n, 1)))
+
+
+def judge(ids, w, rid, rw):
+    torch.cuda.synchronize()
     assert ids.dtype == torch.int32 and tuple(ids.shape) == rid.shape
     got = ids.cpu().numpy()
     bad = np.nonzero((got != rid).any(axis=1))[0]
