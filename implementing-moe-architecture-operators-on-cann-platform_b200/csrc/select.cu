@@ -381,32 +381,35 @@ struct SelBest {
     int e;
 };
 
-// Whether x comes before y, by the difference of their keys:
-//   logits   l_x - l_y;
-//   sigmoid  s_x - s_y = s_x (1 - s_y) (1 - e^-(l_x - l_y));
-//   softmax  s_x - s_y = s_y (e^(l_x - l_y) - 1);
-// plus b_x - b_y.  The first part is known to c of itself (the errors of two scores, as
-// bounded in the kernel, and of expm1), the second to 2^-24.  `lost` is set where that does
-// not decide.
+// Whether x comes before y, by the difference of their keys.  With h the one of the larger
+// logit, o the other and d = l_h - l_o (nothing here can overflow, and what underflows is
+// below 1e-36):
+//   sigmoid  s_h - s_o = s_h (1 - s_o) (1 - e^-d)
+//   softmax  s_h - s_o = s_h (1 - e^-d)
+// plus the difference of their biases.  The first part is known to c of itself (the errors
+// of the scores, as bounded in the kernel, and of expm1), the second to 2^-24.  `lost` is
+// set where that does not decide, and for differences that 64-bit keys would round away.
 __device__ __forceinline__ bool sel_before(const SelectArgs& a, bool by_logit, const SelBest& x, const SelBest& y, float mx,
                                            float inv, bool& lost)
 {
     const bool id = x.e < y.e;
     if (by_logit) return x.l > y.l || (x.l == y.l && id);
     if (x.l == y.l && x.b == y.b) return id;
-    const float d = x.l - y.l;
     float A = 0.0f, c = 0.0f;
-    if (d != 0.0f) {
+    if (x.l != y.l) {
+        const float h = fmaxf(x.l, y.l), o = fminf(x.l, y.l);
+        A = -expm1f(o - h);
         if (a.sigmoid) {
-            A = -expm1f(-d) * sel_rcp(1.0f + sel_ex2(x.l * -SEL_LOG2E)) * sel_rcp(1.0f + sel_ex2(y.l * SEL_LOG2E));
-            c = fmaxf(fabsf(x.l), fabsf(y.l)) * 4e-7f + 3e-6f;
+            A *= sel_rcp(1.0f + sel_ex2(h * -SEL_LOG2E)) * sel_rcp(1.0f + sel_ex2(o * SEL_LOG2E));
+            c = fmaxf(fabsf(h), fabsf(o)) * 4e-7f + 3e-6f;
         } else {
-            A = expm1f(d) * sel_ex2((y.l - mx) * SEL_LOG2E) * inv;
-            c = (mx - y.l) * 2.5e-7f + 3e-6f;
+            A *= h == mx ? inv : sel_ex2((h - mx) * SEL_LOG2E) * inv;
+            c = (h == mx ? 0.0f : mx - h) * 2.5e-7f + 3e-6f;
         }
+        if (y.l > x.l) A = -A;
     }
     const float B = x.b - y.b, D = A + B;
-    lost |= !(fabsf(D) > fabsf(A) * c + fabsf(B) * 2.4e-7f + 1e-36f);
+    lost |= !(fabsf(D) > fabsf(A) * c + fabsf(B) * 2.4e-7f + (1.0f + fmaxf(fabsf(x.b), fabsf(y.b))) * 1e-15f);
     return D > 0.0f;
 }
 
@@ -600,7 +603,9 @@ __global__ void __launch_bounds__(SEL_WARPS * 32, 5) select_kernel(const SelectA
             // ---- slot r's key to lane r, and the two keys after the last slot
             float win = SEL_NINF, after1 = SEL_NINF, after2 = SEL_NINF;
             if constexpr (LPT == 32) {
-                // the largest head, K + 2 times
+                // the largest head, K + 2 times; a lane whose list runs out has lost sight of
+                // what comes after it
+                const bool full = p.per_lane > 8 && v8[7] > SEL_NINF;
 #pragma unroll 1
                 for (int r = 0; r < a.K + 2; r++) {
                     const float m = warp_max(v8[0]);
@@ -613,6 +618,7 @@ __global__ void __launch_bounds__(SEL_WARPS * 32, 5) select_kernel(const SelectA
                         v8[7] = SEL_NINF;
                     }
                 }
+                dark |= full && v8[0] == SEL_NINF;
             } else {
                 // lists merge pairwise until every lane has the token's eight largest
                 float t8[8];
@@ -690,6 +696,11 @@ __global__ void __launch_bounds__(SEL_WARPS * 32, 5) select_kernel(const SelectA
                         at = a.K - __popc((less >> shift) & MASK);
                         dark |= !(after1 > SEL_CLOSED && sel_open(l));
                     }
+                    // every slot is taken once, or the comparisons were not of one order
+                    unsigned taken = slot ? 1u << at : 0u;
+#pragma unroll
+                    for (int d = LPT / 2; d; d >>= 1) taken |= __shfl_xor_sync(0xffffffffu, taken, d);
+                    dark |= taken != (1u << a.K) - 1u;
                 }
             }
             const float w = sel_weight<LPT>(a, l, slot, mx, total);

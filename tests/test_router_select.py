@@ -156,6 +156,13 @@ def test_scores_closer_than_32_bits_tell_apart(moe, gpu, score):
             check(moe, logits, K, torch.float32, bias=bias, score=score, renorm=renorm)
             check(moe, logits, K, torch.float32, bias=bias, score=score, renorm=renorm, G=8, topG=3, groupTop=2)
             check(moe, logits, K, torch.float32, bias=bias, score=score, renorm=renorm, G=8, topG=3, groupTop=1)
+    # one group of 15, one lane's work, that holds every slot and what comes after
+    order = torch.stack([torch.randperm(255, generator=g) for _ in range(T)])
+    logits = (base.double() + order.double() * ulp.double()).float().cuda()
+    for K in (6, 7, 8):
+        for bias in (None, torch.full((255,), 0.25).cuda()):
+            check(moe, logits, K, torch.float32, bias=bias, score=score, G=17, topG=1, groupTop=2)
+            check(moe, logits, K, torch.float32, bias=bias, score=score, G=17, topG=1, groupTop=1)
 
 
 @pytest.mark.gpu
@@ -214,6 +221,22 @@ def test_small_scores_keep_their_ratio(moe, gpu):
     check(moe, l, 5, torch.float32, score="sigmoid", renorm=True)
     check(moe, l, 5, torch.float32, score="sigmoid", renorm=True, bias=torch.zeros(40).cuda())
     check(moe, l, 5, torch.float32, score="softmax", renorm=True, bias=torch.zeros(40).cuda())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_scores_from_one_to_underflow(moe, gpu, score):
+    """Logits over a hundred units, so that scores of one row lie between 1 and what fp32
+    cannot hold, beside biases of a thousandth: every comparison among the best must agree
+    with every other, or a slot stays unwritten."""
+    for i, (T, E, K, G, topG, groupTop) in enumerate([(150, 64, 8, 1, 1, 1), (120, 64, 8, 16, 6, 1), (100, 256, 8, 8, 4, 2),
+                                                      (100, 250, 7, 5, 3, 2), (100, 128, 4, 2, 2, 2),
+                                                      (150, 255, 8, 17, 1, 2), (150, 255, 7, 17, 1, 2)]):
+        g = torch.Generator().manual_seed(i)
+        l = (torch.randn((T, E), generator=g) * 20 - 30 + 10 * (i % 3)).cuda()
+        b = (torch.randn(E, generator=g) * 10.0 ** -(3 + i % 3)).cuda()
+        for renorm in (False, True):
+            check(moe, l, K, torch.float32, bias=b, G=G, topG=topG, groupTop=groupTop, score=score, renorm=renorm)
 
 
 @pytest.mark.gpu
