@@ -184,10 +184,11 @@ __device__ __noinline__ int select_exact(const SelectArgs& a, const LT* row, Exa
 // What the lost bits or the fast exp and quotient may have turned around is noticed.
 // Neighbours among the K + 1 best closer than the bounds below are compared once more by the
 // difference of their keys (sel_before), which fp32 knows to a few millionths of itself.
-// Groups too close, a closed expert among those that count, or differences that cancel send
-// the token to a list, which select_slow settles in 64 bits when the warp is through.
+// Groups too close, or differences that cancel, send the token to a list, which select_slow
+// settles in 64 bits when the warp is through.  Closed experts are looked for only where one
+// turns up among the keys that count: the tokens of the warp are then done over, with care.
 constexpr float SEL_MAX = 3.4028235e38f;
-constexpr float SEL_CLOSED = -3.4e38f;  // keys at or below: closed, or as low as can be
+constexpr float SEL_CLOSED = -3.4e38f;  // keys at or below may be closed experts' 
 #define SEL_NINF (-CUDART_INF_F)
 
 template <int LPT>
@@ -423,7 +424,7 @@ struct SelectPlan {
 constexpr int SEL_LIST = 32;
 
 template <typename LT, int LPT, bool WHOLE>
-__global__ void __launch_bounds__(SEL_WARPS * 32, 5) select_kernel(const SelectArgs a, const SelectPlan p)
+__global__ void __launch_bounds__(SEL_WARPS * 32, 5) select_kernel(const __grid_constant__ SelectArgs a, const __grid_constant__ SelectPlan p)
 {
     constexpr int TPW = 32 / LPT;              // tokens per warp
     constexpr bool EXACT16 = sizeof(LT) == 2;  // a 16-bit logit is whole in the upper 24 bits
@@ -440,7 +441,7 @@ __global__ void __launch_bounds__(SEL_WARPS * 32, 5) select_kernel(const SelectA
     const int sub = lane & (LPT - 1), tok = lane / LPT, shift = tok * (LPT & 31);
     if (a.bias) {
         for (int e = threadIdx.x; e < a.E; e += SEL_WARPS * 32)
-            *reinterpret_cast<float*>(sbias + sel_at<WHOLE>(e * 4)) = fminf(fmaxf(a.bias[e], -SEL_MAX), SEL_MAX);
+            *reinterpret_cast<float*>(sbias + sel_at<WHOLE>(e * 4)) = sel_open(a.bias[e]) ? fminf(a.bias[e], SEL_MAX) : SEL_NINF;
         __syncthreads();
     }
     const int size = a.E / a.G;
@@ -501,98 +502,19 @@ __global__ void __launch_bounds__(SEL_WARPS * 32, 5) select_kernel(const SelectA
             const float sign = mx > 0.0f ? 1.0f : -1.0f;  // a sigmoid's keys: s - 1 or s
             // ---- keys, eight at a time, merged into this lane's eight largest
             float v8[8];
-#pragma unroll 1
-            for (int c = 0; c < p.per_lane; c += 8) {
-                float v[8];
-                sel_chunk<WHOLE, LT>(v, row, first + c, mine - c, SEL_NINF);
-                const int id = 255 - (first + c);
-                if (p.by_logit) {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        // the lower id ahead: more in the low bits of a positive number is
-                        // more, of a negative one less; + 0 makes one zero of two
-                        const int b = __float_as_int(fminf(fmaxf(v[i] + 0.0f, -SEL_MAX), SEL_MAX));
-                        v[i] = __int_as_float((b & ~255) | (((b >> 31) ^ (id - i)) & 255));
-                    }
-                } else {
-                    if (a.sigmoid) {
-#pragma unroll
-                        for (int i = 0; i < 8; i++) v[i] = -sign * sel_rcp(1.0f + sel_ex2(v[i] * (sign * SEL_LOG2E)));
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; i++) v[i] = (v[i] == mx ? 1.0f : sel_ex2((v[i] - mx) * SEL_LOG2E)) * inv;
-                    }
-                    if (a.bias) {
-                        float b[8];
-                        sel_chunk<WHOLE, float>(b, sbias, first + c, mine - c, 0.0f);
-#pragma unroll
-                        for (int i = 0; i < 8; i++) v[i] += b[i];
-                    }
-#pragma unroll
-                    for (int i = 0; i < 8; i++)  // (NaN becomes -SEL_MAX)
-                        v[i] = __int_as_float((__float_as_int(fmaxf(v[i], -SEL_MAX)) & ~255) | ((id - i) & 255));
-                }
-                if (!WHOLE) {
-#pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        if (c + i >= mine) v[i] = SEL_NINF;
-                }
-                sel_sort<8>(v);
-                if (c == 0) {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) v8[i] = v[i];
-                } else {
-                    sel_merge8(v8, v);
-                }
-            }
             bool dark = false;  // for select_slow
-            // ---- groups
-            if (a.G > 1) {
-                float m1 = v8[0], m2 = v8[1];
-                for (int d = (1 << p.shift) >> 1; d; d >>= 1) {
-                    const float o1 = __shfl_xor_sync(0xffffffffu, m1, d), o2 = __shfl_xor_sync(0xffffffffu, m2, d);
-                    m2 = fmaxf(fminf(m1, o1), fmaxf(m2, o2));
-                    m1 = fmaxf(m1, o1);
-                }
-                // the low bits must not count: they are ids
-                const int b1 = __float_as_int(m1), b2 = __float_as_int(m2);
-                const float k1 = __int_as_float(b1 & ~255), k2 = __int_as_float(b2 & ~255);
-                float val = SEL_NINF, mag = 0.0f;
-                if (grp < a.G) {
-                    val = a.groupTop > 1 ? fmaxf(k1 + k2, -SEL_MAX) : k1;
-                    mag = fabsf(k1) + (a.groupTop > 1 ? fabsf(k2) : 0.0f);
-                    // the group's best, or second best, is closed: its value is another
-                    const int e1 = p.by_logit && b1 < 0 ? b1 & 255 : 255 - (b1 & 255), e2 = 255 - (b2 & 255);
-                    dark = !(m1 > SEL_CLOSED && sel_open(sel_get<WHOLE, LT>(row, e1)));
-                    if (a.groupTop > 1) dark |= !(m2 > SEL_CLOSED && sel_open(sel_get<WHOLE, LT>(row, e2)));
-                }
-                int before = 0;
-                for (int d = 1 << p.shift; d < LPT; d += 1 << p.shift) {
-                    const int from = sub ^ d;
-                    const float o = __shfl_xor_sync(0xffffffffu, val, d);
-                    before += (o > val || (o == val && (from >> p.shift) < grp)) ? 1 : 0;
-                }
-                const bool stay = before < a.topG;
-                if (!exact) {
-                    const float in = -sub_max<LPT>(stay ? -val : SEL_NINF);  // the least that stays
-                    const float out = sub_max<LPT>(stay ? SEL_NINF : val);   // the most that does not
-                    // Each key is off by 2^-15 of its size (the bits given to ids) and by its
-                    // score's error: 2^-15 of it, and 2e-6 at most, a sigmoid's 5e-7 (see
-                    // below); two keys on either side.
-                    float tol;
-                    if (a.sigmoid || a.bias)
-                        tol = sub_max<LPT>(mag) * 6.2e-5f + (a.sigmoid ? 2e-6f : 8e-6f);
-                    else
-                        tol = (fabsf(in) + fabsf(out)) * 6.6e-5f + 1e-37f;
-                    dark |= out > SEL_NINF && !(in - out > tol);
-                }
-                if (!stay) {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) v8[i] = SEL_NINF;
-                }
-            }
-            // the largest of the token's keys below x (LPT = 8); a lane whose eight are all not
-            // below has lost sight of its own next
+            bool stay = true;   // this lane's group
+            float win, after1, after2;
+            // the expert of a key, and the key without its id
+            auto expert = [&](float key) {
+                const int b = __float_as_int(key);
+                return !(key > SEL_NINF) ? 0 : (p.by_logit && b < 0 ? b & 255 : 255 - (b & 255));
+            };
+            auto value = [&](float key) { return key > SEL_NINF ? __int_as_float(__float_as_int(key) & ~255) : SEL_NINF; };
+            // a key that counts may be a closed expert's
+            auto suspect = [&](float key) { return !(key > SEL_CLOSED && sel_open(sel_get<WHOLE, LT>(row, expert(key)))); };
+            // the largest of the token's keys below x; a lane whose eight are all not below has
+            // lost sight of its own next
             auto below = [&](float x) {
                 float m = SEL_NINF;
 #pragma unroll
@@ -600,56 +522,156 @@ __global__ void __launch_bounds__(SEL_WARPS * 32, 5) select_kernel(const SelectA
                 dark |= p.per_lane > 8 && v8[7] > SEL_NINF && v8[7] >= x;
                 return sub_max<LPT>(m);
             };
-            // ---- slot r's key to lane r, and the two keys after the last slot
-            float win = SEL_NINF, after1 = SEL_NINF, after2 = SEL_NINF;
-            if constexpr (LPT == 32) {
-                // the largest head, K + 2 times; a lane whose list runs out has lost sight of
-                // what comes after it
-                const bool full = p.per_lane > 8 && v8[7] > SEL_NINF;
 #pragma unroll 1
-                for (int r = 0; r < a.K + 2; r++) {
-                    const float m = warp_max(v8[0]);
-                    if (sub == r) win = m;
-                    after1 = after2;
-                    after2 = m;
-                    if (__float_as_int(v8[0]) == __float_as_int(m)) {  // (bits: -0 is not +0)
+            for (int careful = 0;; careful++) {
+                bool shut = false;
+                dark = false;
+                win = after1 = after2 = SEL_NINF;
+#pragma unroll 1
+                for (int c = 0; c < p.per_lane; c += 8) {
+                    float v[8];
+                    sel_chunk<WHOLE, LT>(v, row, first + c, mine - c, SEL_NINF);
+                    const int id = 255 - (first + c);
+                    unsigned closed = 0;
+                    if (careful) {
 #pragma unroll
-                        for (int i = 0; i < 7; i++) v8[i] = v8[i + 1];
-                        v8[7] = SEL_NINF;
+                        for (int i = 0; i < 8; i++) closed |= (sel_open(v[i]) ? 0u : 1u) << i;
+                    }
+                    if (p.by_logit) {
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            // the lower id ahead: more in the low bits of a positive number is
+                            // more, of a negative one less; + 0 makes one zero of two
+                            const int b = __float_as_int(fminf(fmaxf(v[i] + 0.0f, -SEL_MAX), SEL_MAX));
+                            v[i] = __int_as_float((b & ~255) | (((b >> 31) ^ (id - i)) & 255));
+                        }
+                    } else {
+                        if (a.sigmoid) {
+#pragma unroll
+                            for (int i = 0; i < 8; i++) v[i] = -sign * sel_rcp(1.0f + sel_ex2(v[i] * (sign * SEL_LOG2E)));
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 8; i++) v[i] = (v[i] == mx ? 1.0f : sel_ex2((v[i] - mx) * SEL_LOG2E)) * inv;
+                        }
+                        if (a.bias) {
+                            float b[8];
+                            sel_chunk<WHOLE, float>(b, sbias, first + c, mine - c, 0.0f);
+#pragma unroll
+                            for (int i = 0; i < 8; i++) v[i] += b[i];
+                            if (careful) {
+#pragma unroll
+                                for (int i = 0; i < 8; i++) closed |= (sel_open(b[i]) ? 0u : 1u) << i;
+                            }
+                        }
+#pragma unroll
+                        for (int i = 0; i < 8; i++)  // (NaN becomes -SEL_MAX)
+                            v[i] = __int_as_float((__float_as_int(fmaxf(v[i], -SEL_MAX)) & ~255) | ((id - i) & 255));
+                    }
+                    if (!WHOLE) closed |= 0xffu << max(0, min(mine - c, 8));
+                    if (!WHOLE || careful) {
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+                            if ((closed >> i) & 1u) v[i] = SEL_NINF;
+                    }
+                    sel_sort<8>(v);
+                    if (c == 0) {
+#pragma unroll
+                        for (int i = 0; i < 8; i++) v8[i] = v[i];
+                    } else {
+                        sel_merge8(v8, v);
                     }
                 }
-                dark |= full && v8[0] == SEL_NINF;
-            } else {
-                // lists merge pairwise until every lane has the token's eight largest
-                float t8[8];
+                // ---- groups
+                if (a.G > 1) {
+                    float m1 = v8[0], m2 = v8[1];
+                    for (int d = (1 << p.shift) >> 1; d; d >>= 1) {
+                        const float o1 = __shfl_xor_sync(0xffffffffu, m1, d), o2 = __shfl_xor_sync(0xffffffffu, m2, d);
+                        m2 = fmaxf(fminf(m1, o1), fmaxf(m2, o2));
+                        m1 = fmaxf(m1, o1);
+                    }
+                    const float k1 = value(m1), k2 = value(m2);
+                    float val = SEL_NINF, mag = 0.0f;
+                    if (m1 > SEL_NINF) {
+                        const bool two = a.groupTop > 1 && m2 > SEL_NINF;
+                        // (one key where others have two: 1 less, if theirs are 1 less each)
+                        const float alone = a.groupTop > 1 && !two && a.sigmoid && sign > 0.0f ? 1.0f : 0.0f;
+                        val = two ? fmaxf(k1 + k2, -SEL_MAX) : k1 - alone;
+                        mag = fabsf(k1) + (two ? fabsf(k2) : alone);
+                        shut = suspect(m1) || (two && suspect(m2));
+                    }
+                    int before = 0;
+                    for (int d = 1 << p.shift; d < LPT; d += 1 << p.shift) {
+                        const int from = sub ^ d;
+                        const float o = __shfl_xor_sync(0xffffffffu, val, d);
+                        before += (o > val || (o == val && (from >> p.shift) < grp)) ? 1 : 0;
+                    }
+                    stay = before < a.topG;
+                    if (!exact) {
+                        const float in = -sub_max<LPT>(stay ? -val : SEL_NINF);  // the least that stays
+                        const float out = sub_max<LPT>(stay ? SEL_NINF : val);   // the most that does not
+                        // Each key is off by 2^-15 of its size (the bits given to ids) and by its
+                        // score's error: 2^-15 of it, and 2e-6 at most, a sigmoid's 5e-7 (see
+                        // below); two keys on either side.
+                        float tol;
+                        if (a.sigmoid || a.bias)
+                            tol = sub_max<LPT>(mag) * 6.2e-5f + (a.sigmoid ? 2e-6f : 8e-6f);
+                        else
+                            tol = (fabsf(in) + fabsf(out)) * 6.6e-5f + 1e-37f;
+                        dark |= out > SEL_NINF && !(in - out > tol);
+                    }
+                    if (!stay) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) t8[i] = v8[i];
+                        for (int i = 0; i < 8; i++) v8[i] = SEL_NINF;
+                    }
+                }
+                // ---- slot r's key to lane r, and the two keys after the last slot
+                if constexpr (LPT == 32) {
+                    // the largest head, K + 2 times; a lane whose list runs out has lost sight of
+                    // what comes after it
+                    const bool full = p.per_lane > 8 && v8[7] > SEL_NINF;
 #pragma unroll 1
-                for (int d = 1; d < LPT; d *= 2) {
-                    float o[8];
+                    for (int r = 0; r < a.K + 2; r++) {
+                        const float m = warp_max(v8[0]);
+                        if (sub == r) win = m;
+                        after1 = after2;
+                        after2 = m;
+                        if (__float_as_int(v8[0]) == __float_as_int(m)) {  // (bits: -0 is not +0)
 #pragma unroll
-                    for (int i = 0; i < 8; i++) o[i] = __shfl_xor_sync(0xffffffffu, t8[i], d);
-                    sel_merge8(t8, o);
-                }
+                            for (int i = 0; i < 7; i++) v8[i] = v8[i + 1];
+                            v8[7] = SEL_NINF;
+                        }
+                    }
+                    dark |= full && v8[0] == SEL_NINF;
+                } else {
+                    // lists merge pairwise until every lane has the token's eight largest
+                    float t8[8];
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    if (sub == i) win = t8[i];
-                    if (a.K == i) after1 = t8[i];
-                    if (a.K + 1 == i) after2 = t8[i];
+                    for (int i = 0; i < 8; i++) t8[i] = v8[i];
+#pragma unroll 1
+                    for (int d = 1; d < LPT; d *= 2) {
+                        float o[8];
+#pragma unroll
+                        for (int i = 0; i < 8; i++) o[i] = __shfl_xor_sync(0xffffffffu, t8[i], d);
+                        sel_merge8(t8, o);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        if (sub == i) win = t8[i];
+                        if (a.K == i) after1 = t8[i];
+                        if (a.K + 1 == i) after2 = t8[i];
+                    }
+                    // the ninth: the largest below the eighth
+                    if (a.K == 8) after1 = below(t8[7]);
+                    if (a.K == 7) after2 = below(t8[7]);
                 }
-                // the ninth: the largest below the eighth
-                if (a.K == 8) after1 = below(t8[7]);
-                if (a.K == 7) after2 = below(t8[7]);
+                if (sub < a.K) shut |= suspect(win);
+                if (after1 > SEL_NINF) shut |= suspect(after1);
+                if (careful || !__any_sync(0xffffffffu, shut)) break;
             }
-            const bool slot = sub < a.K;
-            auto expert = [&](float key) {
-                const int b = __float_as_int(key);
-                return !(key > SEL_NINF) ? 0 : (p.by_logit && b < 0 ? b & 255 : 255 - (b & 255));
-            };
-            auto value = [&](float key) { return key > SEL_NINF ? __int_as_float(__float_as_int(key) & ~255) : SEL_NINF; };
+            const bool slot = sub < a.K && win > SEL_NINF;
+            const int open = __popc((__ballot_sync(0xffffffffu, slot) >> shift) & MASK);  // slots with an open expert
             int e = slot ? expert(win) : 0, at = sub;
             float l = sel_get<WHOLE, LT>(row, e);
-            if (slot) dark |= !(win > SEL_CLOSED && sel_open(l));
             if (!exact) {
                 // Two keys with truncated values this far apart are in order: a step of the
                 // truncation (2^-15 of the key) and twice a score's error.  A sigmoid is off
@@ -666,7 +688,7 @@ __global__ void __launch_bounds__(SEL_WARPS * 32, 5) select_kernel(const SelectA
                 if (__any_sync(0xffffffffu, doubt)) {
                     // compare once more, everyone with everyone and with the one after
                     if (LPT == 8 && a.K == 8) after2 = below(after1);
-                    if (sub == a.K - 1 && doubt) dark |= !apart(value(after1), value(after2));  // a third at the border
+                    if (slot && sub == a.K - 1 && doubt) dark |= !apart(value(after1), value(after2));  // a third at the border
                     const SelBest me = {l, a.bias ? sel_get<WHOLE, float>(sbias, e) : 0.0f, e};
                     SelBest other;
                     bool lost = false, beaten = false;
@@ -683,7 +705,7 @@ __global__ void __launch_bounds__(SEL_WARPS * 32, 5) select_kernel(const SelectA
                             other.b = a.bias ? sel_get<WHOLE, float>(sbias, other.e) : 0.0f;
                         }
                         beaten = false;
-                        if (j != sub && (j < a.K || after1 > SEL_NINF))
+                        if (j != sub && (j < a.K ? j < open : after1 > SEL_NINF))
                             beaten = sel_before(a, p.by_logit, other, me, mx, inv, lost);
                         before += beaten ? 1 : 0;
                     }
@@ -694,18 +716,39 @@ __global__ void __launch_bounds__(SEL_WARPS * 32, 5) select_kernel(const SelectA
                         e = other.e;
                         l = other.l;
                         at = a.K - __popc((less >> shift) & MASK);
-                        dark |= !(after1 > SEL_CLOSED && sel_open(l));
                     }
                     // every slot is taken once, or the comparisons were not of one order
                     unsigned taken = slot ? 1u << at : 0u;
 #pragma unroll
                     for (int d = LPT / 2; d; d >>= 1) taken |= __shfl_xor_sync(0xffffffffu, taken, d);
-                    dark |= taken != (1u << a.K) - 1u;
+                    dark |= taken != (1u << open) - 1u;
                 }
             }
             const float w = sel_weight<LPT>(a, l, slot, mx, total);
             const unsigned darks = __ballot_sync(0xffffffffu, dark);
-            if (slot && t0 + tok < T && !((darks >> shift) & MASK)) sel_store(a, t, at, e, w);
+            const bool done = t0 + tok < T && !((darks >> shift) & MASK);
+            if (slot && done) sel_store(a, t, at, e, w);
+            if (__any_sync(0xffffffffu, open < a.K)) {
+                // closed experts fill the slots that are left, lowest id first
+                auto shut = [&](int i) {
+                    return !(stay && sel_open(sel_get<WHOLE, LT>(row, first + i)) &&
+                             (!a.bias || sel_open(sel_get<WHOLE, float>(sbias, first + i))));
+                };
+                int n = 0;
+                for (int i = 0; i < mine; i++) n += shut(i) ? 1 : 0;
+                int m = n;  // those of the lanes up to this one
+#pragma unroll
+                for (int d = 1; d < LPT; d *= 2) {
+                    const int o = __shfl_up_sync(0xffffffffu, m, d, LPT);
+                    if (sub >= d) m += o;
+                }
+                int pos = open + m - n;
+                for (int i = 0; i < mine && pos < a.K; i++)
+                    if (shut(i)) {
+                        if (done) sel_store(a, t, pos, first + i, 0.0f);
+                        pos++;
+                    }
+            }
             if (darks) {
 #pragma unroll 1
                 for (int k = 0; k < TPW && t0 + k < T; k++)

@@ -214,6 +214,25 @@ def test_masked_experts_and_rows(moe, gpu, score, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_groups_with_few_open_experts(moe, gpu, score):
+    """Random masks that leave groups with none, one or a few open experts, by the logit, the
+    bias or both; scores near 1, near a half and near 0."""
+    for i, (T, E, K, G, topG, groupTop) in enumerate([(120, 64, 8, 8, 2, 2), (100, 160, 8, 32, 13, 2), (100, 256, 5, 16, 6, 2),
+                                                      (100, 250, 8, 5, 3, 2), (100, 60, 4, 4, 2, 1), (100, 64, 7, 4, 3, 2)]):
+        for off in (8.0, 0.0, -6.0):
+            g = torch.Generator().manual_seed(10 * i)
+            l = torch.randn((T, E), generator=g) * 1.5 + off
+            keep = torch.rand((T, E), generator=g) < torch.rand((T, 1), generator=g)
+            l = torch.where(keep, l, -INF).cuda()
+            b = steps_bias(E, i)
+            for dtype in (torch.float32, torch.bfloat16):
+                check(moe, l.to(dtype), K, torch.float32, G=G, topG=topG, groupTop=groupTop, score=score, renorm=True)
+            b[torch.randperm(E, generator=g)[: E // 2].cuda()] = -INF
+            check(moe, l, K, torch.float32, bias=b, G=G, topG=topG, groupTop=groupTop, score=score)
+
+
+@pytest.mark.gpu
 def test_small_scores_keep_their_ratio(moe, gpu):
     """Sigmoids that underflow in 32 bits still renormalise to their ratio."""
     g = torch.Generator().manual_seed(3)
