@@ -239,19 +239,19 @@ constexpr int LG_GROUP_M = 8;                  // m tiles that run together over
 // own 128 tokens and one 128-row half of w.
 template <int PAIR, int BN>
 struct LinCfg {
-    static_assert(BN == 256 || (BN == 128 && !PAIR), "tile");
+    static_assert(BN == 256 || BN == 128, "tile");
     static constexpr int B_HALF = (BN / 2) * LG_BK * 2;  // bytes of one box of w
     static constexpr int KB_BYTES = LG_A_BYTES + (PAIR ? B_HALF : 2 * B_HALF);
     // k blocks per stage: with 128 columns the four UMMAs of one run for 256 cycles, little
     // more than their issue, commit and wait
     static constexpr int KPS = BN == 128 ? 2 : 1;
     static constexpr int STAGE_BYTES = KPS * KB_BYTES;
-    static constexpr int STAGES = PAIR ? 6 : (BN == 256 ? 4 : 3);
+    static constexpr int STAGES = PAIR ? (BN == 256 ? 6 : 4) : (BN == 256 ? 4 : 3);
     static constexpr int ROWS = PAIR ? 2 * LG_BM : LG_BM;
     static constexpr uint32_t TMEM_COLS = 2 * BN;
     // A copy takes about 95 cycles to issue; a k block of a narrow tile runs 256 and needs
     // three: x then has a warp of its own.
-    static constexpr bool X_WARP = BN == 128;
+    static constexpr bool X_WARP = BN == 128 && !PAIR;
     static constexpr int THREADS = LG_THREADS + (X_WARP ? 32 : 0);
 };
 
@@ -279,7 +279,7 @@ __host__ __device__ constexpr size_t lin_smem_bytes()
     return 1024 + (size_t)LinCfg<PAIR, BN>::STAGES * LinCfg<PAIR, BN>::STAGE_BYTES + LG_TAIL + LG_EPI_WARPS * LG_STG_WARP;
 }
 static_assert(lin_smem_bytes<1, 256>() <= 227 * 1024 && lin_smem_bytes<0, 256>() <= 227 * 1024 &&
-                  lin_smem_bytes<0, 128>() <= 227 * 1024, "smem");
+                  lin_smem_bytes<0, 128>() <= 227 * 1024 && lin_smem_bytes<1, 128>() <= 227 * 1024, "smem");
 
 struct LinParams {
     const void* bias;
@@ -541,6 +541,11 @@ linear_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
             tmem_relinquish();
         }
     }
+    // what the producers need first, while TMEM is allocated
+    const uint64_t pol_x = l2_policy_evict_last();
+    const uint64_t pol_w = p.w_evict_first ? l2_policy_evict_first() : l2_policy_evict_last();
+    int m, n;
+    lin_tile(p, (uint32_t)unit, m, n);
     tc_fence_before();
     if (PAIR)
         cluster_sync_all();  // both CTAs' barriers are initialised before any remote arrival
@@ -557,15 +562,12 @@ linear_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
     if (warp == 0 || (Cfg::X_WARP && warp == 2 + LG_EPI_WARPS)) {
         // ---------------------------------------------------------------- producers
         if (elect_one()) {
-            const uint64_t pol_x = l2_policy_evict_last();
-            const uint64_t pol_w = p.w_evict_first ? l2_policy_evict_first() : l2_policy_evict_last();
             const bool do_w = warp == 0, do_x = !Cfg::X_WARP || warp != 0;
             const uint32_t kb_tx = (do_w ? Cfg::KB_BYTES - LG_A_BYTES : 0) + (do_x ? p.x_rows * LG_BK * 2 : 0);
             uint32_t it = 0;
             bool ok = true;
             for (int tile = unit; ok && tile < total; tile += nunits) {
-                int m, n;
-                lin_tile(p, tile, m, n);
+                if (tile != unit) lin_tile(p, tile, m, n);
                 const int x_row = m * ROWS + (int)crank * LG_BM;
                 const int w_lo = n * (p.gated ? BN / 2 : BN);
                 const int w_hi = p.gated ? p.N + w_lo : w_lo + BN / 2;
@@ -581,15 +583,20 @@ linear_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
                     }
                     const uint32_t full = smem_u32(&tail->full[s]);
                     const uint32_t st = smem_u32(smem + s * STAGE_BYTES);
+                    const int nb = min(KPS, nk - kb);
                     if (PAIR) {
                         // both CTAs' copies complete on the leader's barrier, which
                         // expects the bytes of both
                         const uint32_t full_leader = mapa_shared(full, 0);
-                        if (leader) mbar_arrive_expect_tx(full, 2 * kb_tx);
-                        tma_load_2d_pair(st, &tmX, full_leader, kb * LG_BK, x_row, pol_x);
-                        tma_load_2d_pair(st + LG_A_BYTES, &tmW, full_leader, kb * LG_BK, leader ? w_lo : w_hi, pol_w);
+                        if (leader) mbar_arrive_expect_tx(full, 2 * nb * kb_tx);
+#pragma unroll
+                        for (int i = 0; i < KPS; i++) {
+                            if (i >= nb) break;
+                            const uint32_t dst = st + i * Cfg::KB_BYTES;
+                            tma_load_2d_pair(dst, &tmX, full_leader, (kb + i) * LG_BK, x_row, pol_x);
+                            tma_load_2d_pair(dst + LG_A_BYTES, &tmW, full_leader, (kb + i) * LG_BK, leader ? w_lo : w_hi, pol_w);
+                        }
                     } else {
-                        const int nb = min(KPS, nk - kb);
                         mbar_arrive_expect_tx(full, nb * kb_tx);
 #pragma unroll
                         for (int i = 0; i < KPS; i++) {
@@ -688,8 +695,7 @@ linear_gemm_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constan
         const uint32_t tempty0 = PAIR ? mapa_shared(smem_u32(&tail->tempty[0]), 0) : smem_u32(&tail->tempty[0]);
         uint32_t lt = 0;
         for (int tile = unit; tile < total; tile += nunits, lt++) {
-            int m, n;
-            lin_tile(p, tile, m, n);
+            if (tile != unit) lin_tile(p, tile, m, n);
             const uint32_t acc = lt & 1u;
             const uint32_t tpar = (lt >> 1) & 1u;
             const int cols = p.gated ? BN / 2 : BN;
@@ -943,6 +949,9 @@ linear_split_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
     }
     int m, n;
     lin_tile(p, tile, m, n);
+    // (what the producers need first is made while TMEM is allocated)
+    const uint64_t pol_x = l2_policy_evict_last();
+    const uint64_t pol_w = p.w_evict_first ? l2_policy_evict_first() : l2_policy_evict_last();
     // S slabs of 32 rows come for each of the tile's row quarters that exist
     constexpr uint32_t SLAB = 32 * PITCH * 4;
     const int quarters = min(4, (p.T - m * LG_BM + 31) / 32);
@@ -961,7 +970,7 @@ linear_split_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
         // feeds: w (two boxes per k block) and x have a warp each.
         if (elect_one()) {
             const bool is_w = warp == 0;
-            const uint64_t pol = is_w && p.w_evict_first ? l2_policy_evict_first() : l2_policy_evict_last();
+            const uint64_t pol = is_w ? pol_w : pol_x;
             const uint32_t kb_tx = is_w ? 2 * Cfg::B_HALF : p.x_rows * LG_BK * 2;
             const int w_lo = n * cols;
             const int w_hi = p.gated ? p.N + w_lo : w_lo + BN / 2;
@@ -1469,7 +1478,7 @@ SplitChoice choose_split(int T, long long wrows, int nk, int sms)
     return best;
 }
 
-// MOE_LINEAR_TILE=pair|wide|narrow|split2|split4|split8|split2n|split4n|few forces a kernel where
+// MOE_LINEAR_TILE=pair|pairn|wide|narrow|split2|split4|split8|split2n|split4n|few forces a kernel where
 // it can run (few: up to 16 tokens, gated 8; pair and wide: a 16-bit y; splitS: as many k blocks as
 // CTAs; n: 64 columns per tile).
 const char* lin_forced()
@@ -1496,6 +1505,7 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s)
     if (const char* f = lin_forced()) {
         if (!strcmp(f, "few") && (a.T <= 8 || (a.T <= 16 && !a.gated))) return launch_few(a, sms, s);
         if (!strcmp(f, "pair") && !f32) return launch_tiles<1, 256>(a, dev, s);
+        if (!strcmp(f, "pairn") && !f32) return launch_tiles<1, 128>(a, dev, s);
         if (!strcmp(f, "wide") && !f32) return launch_tiles<0, 256>(a, dev, s);
         if (!strcmp(f, "narrow")) return f32 ? launch_tiles<0, 128, true>(a, dev, s) : launch_tiles<0, 128>(a, dev, s);
         if (!strncmp(f, "split", 5) && f[5] >= '2' && f[5] <= '8') {
@@ -1518,6 +1528,11 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s)
     if (mt * nt128 > sms) return f32 ? launch_tiles<0, 128, true>(a, dev, s) : launch_tiles<0, 128>(a, dev, s);
     const SplitChoice c = choose_split(a.T, wrows, nk, sms);
     if (c.S > 1) return launch_split(a, c.S, c.bn, dev, s);
+    // Whole tiles of one wave: 256 x 128 over pairs need 24 KB per CTA and k block where 128 x
+    // 128 need 32, and what SMs take in from L2 bounds these (us): 1024 x 8192 -> 2048 30.2 /
+    // 34.8, 512 x 2048 -> 2048 10.8 / 11.7; with few k blocks the set-up of a pair costs more:
+    // 512 x 512 -> 4096 7.3 / 6.7.
+    if (!f32 && a.T > LG_BM && nk >= 16) return launch_tiles<1, 128>(a, dev, s);
     return f32 ? launch_tiles<0, 128, true>(a, dev, s) : launch_tiles<0, 128>(a, dev, s);
 }
 

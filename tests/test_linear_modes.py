@@ -16,7 +16,7 @@ pytestmark = pytest.mark.gpu
 HERE = os.path.dirname(os.path.abspath(__file__))
 
 
-@pytest.mark.parametrize("mode", ["few", "narrow", "wide", "pair", "split2", "split4", "split8", "split2n", "split4n"])
+@pytest.mark.parametrize("mode", ["few", "narrow", "wide", "pair", "pairn", "split2", "split4", "split8", "split2n", "split4n"])
 def test_each_kernel(mode):
     env = dict(os.environ, MOE_LINEAR_TILE=mode)
     r = subprocess.run([sys.executable, "-m", "pytest", "-q", "-x", "-m", "gpu", "-p", "no:cacheprovider",
