@@ -242,7 +242,7 @@ class _Cuda:
         self.codes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 27}  # MOE_DT_* (include/moe_ops.h)
         self.f32, self.f16, self.i32 = torch.float32, torch.float16, torch.int32
         self.device = torch.cuda.device
-        self.current_device = torch.cuda.current_device
+        self.current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
         # the handle of a device's current stream, without building a Stream object
         raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         self.stream = raw or (lambda index: torch.cuda.current_stream(index).cuda_stream)
@@ -334,9 +334,11 @@ def moe_router_select(logits, topK: int = 2, bias=None, numGroups: int = 1, topG
         wt = 0 if weights.dtype is c.f32 else 1
         if _rows(weights, "weights", T, K, c.f16 if wt else c.f32, dev) != K:
             raise MoeError(-2, "weights must be contiguous")
-    _check(_call_on(dev, lib().MoeRouterSelect, logits.data_ptr(), lt, ldl, None if bias is None else bias.data_ptr(),
-                    expert_ids.data_ptr(), weights.data_ptr(), wt, T, E, K, numGroups, topGroups, groupTop, score,
-                    renormalize, scale), "MoeRouterSelect")
+    rc = _call_on(dev, lib().MoeRouterSelect, logits.data_ptr(), lt, ldl, None if bias is None else bias.data_ptr(),
+                  expert_ids.data_ptr(), weights.data_ptr(), wt, T, E, K, numGroups, topGroups, groupTop, score,
+                  renormalize, scale)
+    if rc:
+        raise MoeError(rc, "MoeRouterSelect")
     return expert_ids, weights
 
 
@@ -379,9 +381,11 @@ def moe_linear(x, weight, bias=None, activation: str = "none", gated: bool = Fal
         raise MoeError(-5, f"y of {ot}")
     ldy = _rows(y, "y", T, N, ot, dev)
     ldr = _rows(residual, "residual", T, N, ot, dev) if residual is not None else 0
-    _check(_call_on(dev, lib().MoeLinear, x.data_ptr(), weight.data_ptr(), None if bias is None else bias.data_ptr(),
-                    None if residual is None else residual.data_ptr(), y.data_ptr(), T, K, N, ldx, ldw, ldr, ldy,
-                    codes[dt], codes[ot], act, gated), "MoeLinear")
+    rc = _call_on(dev, lib().MoeLinear, x.data_ptr(), weight.data_ptr(), None if bias is None else bias.data_ptr(),
+                  None if residual is None else residual.data_ptr(), y.data_ptr(), T, K, N, ldx, ldw, ldr, ldy,
+                  codes[dt], codes[ot], act, gated)
+    if rc:
+        raise MoeError(rc, "MoeLinear")
     return y
 
 
