@@ -261,21 +261,22 @@ def _cu() -> _Cuda:
 def _rows(t, name, rows, cols, dtype, dev):
     """The row stride of a [rows, cols] matrix on `dev` whose rows are contiguous; raises
     MoeError on anything else."""
-    if t.dtype is dtype and t.device == dev and t.shape == (rows, cols) and t.is_contiguous():
-        return cols
+    if t.dtype is dtype and t.device == dev and t.shape == (rows, cols):
+        if t.is_contiguous():
+            return cols
+        across, along = t.stride()
+        if along == 1 or cols <= 1:
+            if rows <= 1:
+                return cols
+            if across >= cols:
+                return across
+            raise MoeError(-2, f"{name}: rows must not overlap")
+        raise MoeError(-2, f"{name}: the elements of a row must be contiguous")
     if t.device != dev:
         raise MoeError(-1, f"{name} must be on {dev} (no CPU fallback), got {t.device}")
     if t.dtype != dtype:
         raise MoeError(-2, f"{name} must be {dtype}, got {t.dtype}")
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
-        raise MoeError(-2, f"{name} must be [{rows}, {cols}], got {list(t.shape)}")
-    if cols > 1 and t.stride(1) != 1:
-        raise MoeError(-2, f"{name}: the elements of a row must be contiguous")
-    if rows <= 1:
-        return cols
-    if t.stride(0) < cols:
-        raise MoeError(-2, f"{name}: rows must not overlap")
-    return t.stride(0)
+    raise MoeError(-2, f"{name} must be [{rows}, {cols}], got {list(t.shape)}")
 
 
 def _vector(t, name, n, dtype, dev):
