@@ -17,6 +17,12 @@
 //       distributed shared memory, and each adds its own slice in rank order;
 //   linear_few_kernel             a few tokens: w is streamed once, straight into the
 //       registers of mma.sync fragments; bound by HBM (by latency for small w).
+// Measured, cold L2, the kernel alone, against the 6515 GB/s of a copy and the 1679 TFLOP/s of
+// a library product: few 8 x 8192 -> 2048 with residual 9.2 us (3.7 TB/s; 128 blocks on 148
+// SMs), split 128 x 2048 -> 2048 8.0 us (latency of the first copies and of the exchange), gemm
+// 128 x 2048 -> 8192 gated 15.1 us (4.6 TB/s), 4096 x 8192 -> 2048 102 us (1351 TFLOP/s; 128
+// tiles on 74 pairs), 8192 x 4096 -> 14336 gated 1229 us (1565 TFLOP/s; tensor pipe, 92% busy
+// on a smaller shape).
 // No atomics, no workspace: the same inputs give the same bits, and calls on different
 // streams share nothing.
 #include <cstdlib>
@@ -1429,18 +1435,24 @@ cudaError_t launch_few_as(const LinearArgs& a, int sms, cudaStream_t s)
 {
     const int rows = a.gated ? 16 : 16 * MT;
     const unsigned grid = (unsigned)((a.N + rows - 1) / rows);
-    // two blocks of 8 warps per SM, or one of 16 where there is no second block
+    // two blocks of 8 warps per SM, or one of 16 where there is no second block.  Measured (us,
+    // 8 / 16 warps): 8 x 8192 -> 2048 10.7 / 9.1, 8 x 2048 -> 2048 4.4 / 4.1, 8 x 2048 -> 3000
+    // 4.5 / 7.0, 8 x 2048 -> 4096 5.0 / 7.4.
     if (grid > (unsigned)sms) return lin_launch(linear_few_kernel<BF16, MT, NT, 8>, grid, 256, 0, 0, s, a);
     return lin_launch(linear_few_kernel<BF16, MT, NT, 16>, grid, 512, 0, 0, s, a);
 }
 
 // At most 8 tokens, or 16 when not gated.  Two blocks of w rows per warp (MT = 2): gated, or
-// rows enough for two blocks on every SM even so.
+// where one block each would take a second wave and two do not.  Measured (us, MT = 1 / 2), 8
+// tokens: 2048 -> 4736 5.2 / 5.6, 2048 -> 5000 6.9 / 6.3, 7168 -> 6144 19.8 / 16.6, 2048 -> 8192
+// 8.9 / 7.2, 2048 -> 9472 9.3 / 7.7; over more waves 7168 -> 12288 31.2 / 33.1, 4096 -> 32768
+// 43.7 / 45.7, 2048 -> 16384 13.9 / 13.5.
 cudaError_t launch_few(const LinearArgs& a, int sms, cudaStream_t s)
 {
     const bool bf16 = a.type == MOE_DT_BF16;
     if (a.T > 8) return bf16 ? launch_few_as<true, 1, 2>(a, sms, s) : launch_few_as<false, 1, 2>(a, sms, s);
-    if (a.gated || a.N >= 64LL * sms) return bf16 ? launch_few_as<true, 2, 1>(a, sms, s) : launch_few_as<false, 2, 1>(a, sms, s);
+    if (a.gated || (a.N > 32LL * sms && a.N <= 64LL * sms))
+        return bf16 ? launch_few_as<true, 2, 1>(a, sms, s) : launch_few_as<false, 2, 1>(a, sms, s);
     return bf16 ? launch_few_as<true, 1, 1>(a, sms, s) : launch_few_as<false, 1, 1>(a, sms, s);
 }
 
@@ -1479,7 +1491,7 @@ SplitChoice choose_split(int T, long long wrows, int nk, int sms)
 }
 
 // MOE_LINEAR_TILE=pair|pairn|wide|narrow|split2|split4|split8|split2n|split4n|few forces a kernel where
-// it can run (few: up to 16 tokens, gated 8; pair and wide: a 16-bit y; splitS: as many k blocks as
+// it can run (few: up to 16 tokens, gated 8; pair, pairn and wide: a 16-bit y; splitS: as many k blocks as
 // CTAs; n: 64 columns per tile).
 const char* lin_forced()
 {
@@ -1525,7 +1537,7 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s)
     // 19.1, gated 512 x 2048 -> 8192 28.7 / 31.8 / 36, gated 128 x 4096 -> 14336 53 / 43 / 47.
     // An fp32 y takes narrow tiles: their warps can hold its sums (see LG_SEGMENT).
     if (mt * nt128 > sms && !f32) return a.T > LG_BM ? launch_tiles<1, 256>(a, dev, s) : launch_tiles<0, 256>(a, dev, s);
-    if (mt * nt128 > sms) return f32 ? launch_tiles<0, 128, true>(a, dev, s) : launch_tiles<0, 128>(a, dev, s);
+    if (mt * nt128 > sms) return launch_tiles<0, 128, true>(a, dev, s);
     const SplitChoice c = choose_split(a.T, wrows, nk, sms);
     if (c.S > 1) return launch_split(a, c.S, c.bn, dev, s);
     // Whole tiles of one wave: 256 x 128 over pairs need 24 KB per CTA and k block where 128 x

@@ -116,6 +116,16 @@ def test_exact_sums_over_shapes(moe, gpu, shape):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("per_sm, more", [(16, -1), (16, 1), (32, 0), (32, 1), (32, 17), (48, 5), (64, 0), (64, 1), (64, 33)])
+def test_exact_sums_where_rows_per_warp_change(moe, gpu, per_sm, more):
+    # a few tokens take one or two blocks of w rows per warp, by how many waves N makes
+    N = per_sm * torch.cuda.get_device_properties(0).multi_processor_count + more
+    for T in (1, 5, 8):
+        check_exact(moe, T, 1032, N, torch.float16, torch.float32, seed=T)
+        check_exact(moe, T, 264, N, torch.bfloat16, torch.bfloat16, act="relu", seed=T + 8)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("act", ["none", "relu", "gelu", "gelu_tanh", "silu", "sigmoid"])
 @pytest.mark.parametrize("gated", [False, True])
 def test_activations(moe, gpu, act, gated):
