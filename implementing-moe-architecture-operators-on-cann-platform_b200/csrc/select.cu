@@ -16,6 +16,10 @@
 // The choice is that of keys in 64 bits: two scores may lie closer together than 32
 // bits tell apart, and the id is a whole number that is right or wrong.  Without a bias
 // scores order as their logits do, so the logits themselves are the keys.
+//
+// Measured, 65536 x 256 fp32 logits, sigmoid, bias, 4 of 8 groups, K = 8: 50 us, 1.4 TB/s.  It
+// reads its 67 MB once; what bounds it is the ALU pipe, on which a min or max takes two issue
+// cycles: 422 instructions per token, 207 of them there, issue slots 61% used.
 #include <math_constants.h>
 
 #include <cuda_bf16.h>
@@ -791,6 +795,10 @@ cudaError_t launch_select_type(const SelectArgs& a, cudaStream_t s)
     p.by_logit = !a.bias && (a.G == 1 || a.groupTop == 1);
     int groups = 1;
     while (groups < a.G) groups *= 2;
+    // Eight lanes per token need a quarter of the merges over lanes, 32 have a quarter of the
+    // chain.  Measured (us, 8 / 32 lanes), 256 experts in 8 groups, T = 256
+    // 7.0 / 5.7, 512 9.1 / 8.3, 1024 11.4 / 11.1, 4096 14.7 / 14.6, 16384 24.0 / 33.5, 65536
+    // 50.1 / 101.5; 64 experts: 512 3.1 / 3.1, 1024 3.1 / 3.8, 4096 4.0 / 6.7, 65536 18 / 68.
     if (groups <= 8 && a.T >= 1024) return launch_select_as<LT, 8>(a, p, groups, s);
     return launch_select_as<LT, 32>(a, p, groups, s);
 }
