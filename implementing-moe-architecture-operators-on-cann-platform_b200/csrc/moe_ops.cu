@@ -500,10 +500,11 @@ int MoeSharedLayerForward(const void* x, const void* w_router, const float* rout
     rc = run_ffn(x, expert_ids, expert_weights, expert_out, T, H, E, K, I, workspace, L.l.f, s, ev,
                  moe::linear_error_word());
     up.err = down.err = at<int>(workspace, L.l.f.p.err);
+    // the shared expert reads x before the combine writes y, which may be x
+    if (rc == MOE_OK && Is > 0) rc = run_linear(up, s);
     if (rc != MOE_OK) return rc;
     rc = cuda_status(moe::launch_combine(static_cast<const __half*>(expert_out), static_cast<const __half*>(weights),
                                          static_cast<__half*>(y), (int)T, (int)H, (int)K, s));
-    if (rc == MOE_OK && Is > 0) rc = run_linear(up, s);
     if (rc == MOE_OK && Is > 0) rc = run_linear(down, s);
     trace_mark(ev, 6, s);
     return rc;

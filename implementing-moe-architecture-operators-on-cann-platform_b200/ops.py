@@ -402,7 +402,8 @@ def moe_shared_layer_forward(x, w_router, expert_weights, shared_gate_up=None, s
     token; returns y [T,H] fp16.
 
     x [T,H], w_router [E,H], expert_weights [E,3I,H], shared_gate_up [2Is,H] and
-    shared_down [H,Is] (both or neither), all contiguous fp16; router_bias [E] fp32."""
+    shared_down [H,Is] (both or neither), all contiguous fp16; router_bias [E] fp32.  y may
+    be x itself."""
     torch = _torch()
     f16 = torch.float16
     for t, name in ((x, "x"), (w_router, "w_router"), (expert_weights, "expert_weights")):

@@ -183,8 +183,8 @@ int MoeLinear(const void* x, const void* weight, const void* bias, const void* r
  * Su), shared_down [H,Is], y [T,H], all fp16; router_bias [E] fp32 or NULL; Is ==
  * sharedSize, a multiple of 8, or 0 without a shared expert (its weights are then NULL).
  * expert_ids [T,K] / weights [T,K] fp16 receive the choice, or are NULL.  The other
- * arguments are MoeRouterSelect's.  The workspace's first word is the device error
- * word (MoeGetDeviceError). */
+ * arguments are MoeRouterSelect's.  y may be x itself, and overlaps nothing else.  The
+ * workspace's first word is the device error word (MoeGetDeviceError). */
 size_t MoeSharedLayerWorkspaceSize(int64_t numTokens, int64_t hiddenSize, int64_t numExperts,
                                    int64_t topK, int64_t intermediateSize, int64_t sharedSize);
 int MoeSharedLayerForward(const void* x, const void* w_router, const float* router_bias,

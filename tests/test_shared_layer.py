@@ -100,6 +100,17 @@ def test_layer_in_a_graph_and_empty(moe, gpu):
     assert tuple(run(moe, (p[0][:0],) + p[1:], K, 4, 2, 2).shape) == (0, H)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", SHAPES)
+def test_layer_in_place(moe, gpu, shape):
+    T, H, E, K, I, Is, G, topG, groupTop = shape
+    p = make(moe, T, H, E, K, I, Is, T)
+    want = run(moe, p, K, G, topG, groupTop)
+    x = p[0].clone()
+    assert run(moe, (x,) + p[1:], K, G, topG, groupTop, y=x) is x
+    assert torch.equal(x, want)
+
+
 def test_refusals_without_gpu(moe):
     L = moe.lib()
     p = 0x10000
