@@ -440,6 +440,10 @@ def moe_shared_layer_forward(x, w_router, expert_weights, shared_gate_up=None, s
         y = torch.empty((T, H), dtype=f16, device=x.device)
     if workspace is None:
         workspace = _workspace(moe_shared_layer_workspace_size(T, H, E, K, I, Is), x.device)
+    else:
+        _cuda(workspace, "workspace", torch.uint8)
+        if workspace.device != x.device:
+            raise MoeError(-1, f"workspace must be on {x.device}, got {workspace.device}")
     _check(_call_on(x.device, lib().MoeSharedLayerForward, _ptr(x), _ptr(w_router), _ptr(router_bias),
                     _ptr(expert_weights), _ptr(shared_gate_up), _ptr(shared_down), _ptr(y), _ptr(expert_ids),
                     _ptr(weights), T, H, E, K, I, Is, numGroups, topGroups, groupTop, SCORE_FUNCS[scoreFunc],

@@ -111,6 +111,16 @@ def test_layer_in_place(moe, gpu, shape):
     assert torch.equal(x, want)
 
 
+@pytest.mark.gpu
+def test_front_end_refuses_a_workspace_the_kernels_cannot_write(moe, gpu):
+    p = make(moe, 4, 64, 8, 2, 64, 32, 1)
+    n = moe.moe_shared_layer_workspace_size(4, 64, 8, 2, 64, 32)
+    for ws in (torch.empty(n, dtype=torch.uint8), torch.empty(2 * n, dtype=torch.uint8, device="cuda")[::2],
+               torch.empty(n, dtype=torch.float32, device="cuda"), torch.empty(n - 1, dtype=torch.uint8, device="cuda")):
+        with pytest.raises(moe.MoeError):
+            run(moe, p, 2, 1, 1, 1, workspace=ws)
+
+
 def test_refusals_without_gpu(moe):
     L = moe.lib()
     p = 0x10000
