@@ -1495,12 +1495,8 @@ SplitChoice choose_split(int T, long long wrows, int nk, int sms)
 // CTAs; n: 64 columns per tile).
 const char* lin_forced()
 {
-#ifdef MOE_LINEAR_TUNE
-    return getenv("MOE_LINEAR_TILE");
-#else
     static const char* v = getenv("MOE_LINEAR_TILE");
     return v;
-#endif
 }
 
 }  // namespace
