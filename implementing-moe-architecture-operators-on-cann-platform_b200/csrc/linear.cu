@@ -1490,58 +1490,109 @@ SplitChoice choose_split(int T, long long wrows, int nk, int sms)
     return best;
 }
 
-// MOE_LINEAR_TILE=pair|pairn|wide|narrow|split2|split4|split8|split2n|split4n|few forces a kernel where
-// it can run (few: up to 16 tokens, gated 8; pair, pairn and wide: a 16-bit y; splitS: as many k blocks as
-// CTAs; n: 64 columns per tile).
-const char* lin_forced()
+// What MOE_LINEAR_TILE may name, and what MoeLinearKernel answers.
+enum LinKind { LIN_NONE, LIN_FEW, LIN_NARROW, LIN_PAIRN, LIN_WIDE, LIN_PAIR, LIN_SPLIT };
+struct LinChoice {
+    LinKind kind;
+    int S, bn;  // LIN_SPLIT only
+    const char* name;
+};
+const LinChoice LIN_CHOICES[] = {
+    {LIN_FEW, 0, 0, "few"},          {LIN_NARROW, 0, 0, "narrow"},    {LIN_PAIRN, 0, 0, "pairn"},
+    {LIN_WIDE, 0, 0, "wide"},        {LIN_PAIR, 0, 0, "pair"},        {LIN_SPLIT, 2, 128, "split2"},
+    {LIN_SPLIT, 4, 128, "split4"},   {LIN_SPLIT, 8, 128, "split8"},   {LIN_SPLIT, 2, 64, "split2n"},
+    {LIN_SPLIT, 4, 64, "split4n"},
+};
+
+LinChoice lin_choice(LinKind kind, int S = 0, int bn = 0)
 {
-    static const char* v = getenv("MOE_LINEAR_TILE");
-    return v;
+    for (const LinChoice& c : LIN_CHOICES)
+        if (c.kind == kind && c.S == S && c.bn == bn) return c;
+    return {LIN_NONE, 0, 0, nullptr};
 }
 
-}  // namespace
-
-cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s)
+// The kernel that MOE_LINEAR_TILE asks for; `bad` when it names none.
+struct LinForced {
+    const LinChoice* choice;
+    bool bad;
+};
+const LinForced& lin_forced()
 {
-    int dev = 0;
-    cudaGetDevice(&dev);
-    const int sms = lin_sm_count(dev);
-    const long long wrows = (long long)a.N * (a.gated ? 2 : 1);
-    const int nk = (a.K + LG_BK - 1) / LG_BK;
-    const bool f32 = a.otype == MOE_DT_FLOAT;
-    const long long mt = (a.T + LG_BM - 1) / LG_BM, nt128 = (wrows + 127) / 128;
-    if (const char* f = lin_forced()) {
-        if (!strcmp(f, "few") && (a.T <= 8 || (a.T <= 16 && !a.gated))) return launch_few(a, sms, s);
-        if (!strcmp(f, "pair") && !f32) return launch_tiles<1, 256>(a, dev, s);
-        if (!strcmp(f, "pairn") && !f32) return launch_tiles<1, 128>(a, dev, s);
-        if (!strcmp(f, "wide") && !f32) return launch_tiles<0, 256>(a, dev, s);
-        if (!strcmp(f, "narrow")) return f32 ? launch_tiles<0, 128, true>(a, dev, s) : launch_tiles<0, 128>(a, dev, s);
-        if (!strncmp(f, "split", 5) && f[5] >= '2' && f[5] <= '8') {
-            int S = f[5] - '0';
-            while (S > nk || (S & (S - 1))) S--;
-            if (S > 1) return launch_split(a, S, strstr(f, "n") ? 64 : 128, dev, s);
+    static const LinForced f = [] {
+        const char* v = getenv("MOE_LINEAR_TILE");
+        if (!v || !*v) return LinForced{nullptr, false};
+        for (const LinChoice& c : LIN_CHOICES)
+            if (!strcmp(c.name, v)) return LinForced{&c, false};
+        return LinForced{nullptr, true};
+    }();
+    return f;
+}
+
+LinChoice choose_linear(int T, int K, int N, bool f32, bool gated, int sms)
+{
+    const long long wrows = (long long)N * (gated ? 2 : 1);
+    const int nk = (K + LG_BK - 1) / LG_BK;
+    const long long mt = (T + LG_BM - 1) / LG_BM, nt128 = (wrows + 127) / 128;
+    const LinForced& f = lin_forced();
+    if (f.bad) return {LIN_NONE, 0, 0, nullptr};
+    if (f.choice) {
+        // where it can run: few up to 16 tokens, gated 8; pair, pairn and wide with a 16-bit
+        // y; a split with as many k blocks as CTAs, or else the largest one that has them
+        const LinChoice& c = *f.choice;
+        if (c.kind == LIN_FEW && (T <= 8 || (T <= 16 && !gated))) return c;
+        if (c.kind == LIN_NARROW) return c;
+        if ((c.kind == LIN_PAIRN || c.kind == LIN_WIDE || c.kind == LIN_PAIR) && !f32) return c;
+        if (c.kind == LIN_SPLIT) {
+            int S = c.S;
+            while (S > nk) S /= 2;
+            if (S > 1) return lin_choice(LIN_SPLIT, S, c.bn);
         }
     }
     // Few tokens.  Measured (us, few / the best of the others): 8 x 2048 -> 2048 4.3 / 6.0,
     // 8 x 8192 -> 2048 9.1 / 13, gated 8 x 4096 -> 14336 40.0 / 40.6.  With two blocks of
     // tokens the registers hold less of w on its way: 16 x 2048 -> 2048 4.5 / 5.8,
     // 16 x 8192 -> 2048 9.7 / 10.9, but 16 x 4096 -> 16384 34 / 26.
-    if (a.T <= 8 || (a.T <= 16 && !a.gated && a.N <= 16 * sms)) return launch_few(a, sms, s);
+    if (T <= 8 || (T <= 16 && !gated && N <= 16 * sms)) return lin_choice(LIN_FEW);
     // At most one wave of 128 x 128 tiles: those, or smaller ones with k split, whichever
     // the model says; else 256 x 256 over CTA pairs, or 128 x 256 where a pair's second half
     // would be empty.  Measured (us, pair / wide / narrow): 2048 x 2048 -> 2048 16.7 / 16.9 /
     // 19.1, gated 512 x 2048 -> 8192 28.7 / 31.8 / 36, gated 128 x 4096 -> 14336 53 / 43 / 47.
     // An fp32 y takes narrow tiles: their warps can hold its sums (see LG_SEGMENT).
-    if (mt * nt128 > sms && !f32) return a.T > LG_BM ? launch_tiles<1, 256>(a, dev, s) : launch_tiles<0, 256>(a, dev, s);
-    if (mt * nt128 > sms) return launch_tiles<0, 128, true>(a, dev, s);
-    const SplitChoice c = choose_split(a.T, wrows, nk, sms);
-    if (c.S > 1) return launch_split(a, c.S, c.bn, dev, s);
+    if (mt * nt128 > sms) return lin_choice(f32 ? LIN_NARROW : T > LG_BM ? LIN_PAIR : LIN_WIDE);
+    const SplitChoice c = choose_split(T, wrows, nk, sms);
+    if (c.S > 1) return lin_choice(LIN_SPLIT, c.S, c.bn);
     // Whole tiles of one wave: 256 x 128 over pairs need 24 KB per CTA and k block where 128 x
     // 128 need 32, and what SMs take in from L2 bounds these (us): 1024 x 8192 -> 2048 30.2 /
     // 34.8, 512 x 2048 -> 2048 10.8 / 11.7; with few k blocks the set-up of a pair costs more:
     // 512 x 512 -> 4096 7.3 / 6.7.
-    if (!f32 && a.T > LG_BM && nk >= 16) return launch_tiles<1, 128>(a, dev, s);
-    return f32 ? launch_tiles<0, 128, true>(a, dev, s) : launch_tiles<0, 128>(a, dev, s);
+    return lin_choice(!f32 && T > LG_BM && nk >= 16 ? LIN_PAIRN : LIN_NARROW);
+}
+
+}  // namespace
+
+const char* linear_kernel_name(int T, int K, int N, bool f32, bool gated)
+{
+    int dev = 0;
+    cudaGetDevice(&dev);
+    return choose_linear(T, K, N, f32, gated, lin_sm_count(dev)).name;
+}
+
+cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s)
+{
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const int sms = lin_sm_count(dev);
+    const bool f32 = a.otype == MOE_DT_FLOAT;
+    const LinChoice c = choose_linear(a.T, a.K, a.N, f32, a.gated != 0, sms);
+    switch (c.kind) {
+        case LIN_FEW: return launch_few(a, sms, s);
+        case LIN_NARROW: return f32 ? launch_tiles<0, 128, true>(a, dev, s) : launch_tiles<0, 128>(a, dev, s);
+        case LIN_PAIRN: return launch_tiles<1, 128>(a, dev, s);
+        case LIN_WIDE: return launch_tiles<0, 256>(a, dev, s);
+        case LIN_PAIR: return launch_tiles<1, 256>(a, dev, s);
+        case LIN_SPLIT: return launch_split(a, c.S, c.bn, dev, s);
+        default: return cudaErrorInvalidValue;  // MOE_LINEAR_TILE names no kernel
+    }
 }
 
 }  // namespace moe

@@ -131,5 +131,8 @@ struct LinearArgs {
 // have no workspace); nullptr if the lookup fails.
 int* linear_error_word();
 cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s);
+// The kernel that launch_linear takes for these sizes, as MOE_LINEAR_TILE names it; nullptr
+// when that variable names none.
+const char* linear_kernel_name(int T, int K, int N, bool f32, bool gated);
 
 }  // namespace moe

@@ -278,7 +278,7 @@ int linear_args(moe::LinearArgs& a, const void* x, const void* w, const void* bi
 int run_linear(const moe::LinearArgs& a, cudaStream_t s)
 {
     cudaError_t e = moe::launch_linear(a, s);
-    if (e == cudaErrorInvalidValue) return MOE_ERR_UNSUPPORTED;  // tensor map rejected
+    if (e == cudaErrorInvalidValue) return MOE_ERR_UNSUPPORTED;  // tensor map rejected, or MOE_LINEAR_TILE
     return cuda_status(e);
 }
 
@@ -449,6 +449,14 @@ int MoeLinear(const void* x, const void* weight, const void* bias, const void* r
     return run_linear(a, static_cast<cudaStream_t>(stream));
 }
 
+const char* MoeLinearKernel(int64_t T, int64_t K, int64_t N, int outDtype, int gated)
+{
+    const int64_t lim = int64_t(1) << 30;
+    if (T < 1 || T > lim || K < 8 || (K & 7) || K > lim || N < 1 || N > lim) return nullptr;
+    if (outDtype != MOE_DT_FLOAT && outDtype != MOE_DT_FLOAT16 && outDtype != MOE_DT_BF16) return nullptr;
+    return moe::linear_kernel_name((int)T, (int)K, (int)N, outDtype == MOE_DT_FLOAT, gated != 0);
+}
+
 size_t MoeSharedLayerWorkspaceSize(int64_t T, int64_t H, int64_t E, int64_t K, int64_t I, int64_t Is)
 {
     if (!ffn_shapes_ok(T, H, E, K, I) || !shared_size_ok(Is)) return 0;
@@ -542,6 +550,7 @@ int MoeGetDeviceError(const void* workspace, int* code, void* stream)
 int MoeRoutingGetDeviceError(int* code, void* stream) { return take_error_word(moe::routing_error_word, code, stream); }
 
 int MoeLinearGetDeviceError(int* code, void* stream) { return take_error_word(moe::linear_error_word, code, stream); }
+
 const char* MoeStatusString(int status)
 {
     switch (status) {

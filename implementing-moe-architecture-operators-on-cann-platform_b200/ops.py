@@ -79,6 +79,8 @@ def lib():
             _int, _int, _int, ctypes.c_float, _vp]
         L.MoeLinear.argtypes = [_vp] * 5 + [_i64] * 7 + [_int] * 4 + [_vp]
         L.MoeLinearGetDeviceError.argtypes = [_intp, _vp]
+        L.MoeLinearKernel.argtypes = [_i64] * 3 + [_int] * 2
+        L.MoeLinearKernel.restype = ctypes.c_char_p
         L.MoeSharedLayerWorkspaceSize.argtypes = [_i64] * 6
         L.MoeSharedLayerWorkspaceSize.restype = _sz
         L.MoeSharedLayerForward.argtypes = [_vp] * 9 + [_i64] * 8 + [_int] * 3 + [ctypes.c_float, _vp, _sz, _vp]
@@ -388,6 +390,14 @@ def moe_linear(x, weight, bias=None, activation: str = "none", gated: bool = Fal
     if rc:
         raise MoeError(rc, "MoeLinear")
     return y
+
+
+def linear_kernel(T: int, K: int, N: int, out_dtype=None, gated: bool = False):
+    """The name of the kernel that moe_linear takes for x [T,K] and y [T,N] on the current
+    device (out_dtype float32 or, by default, 16 bits): a value of MOE_LINEAR_TILE, or None
+    where it refuses the call."""
+    name = lib().MoeLinearKernel(T, K, N, 1 if out_dtype is None else _cu().codes.get(out_dtype, -1), int(bool(gated)))
+    return None if name is None else name.decode()
 
 
 def moe_shared_layer_workspace_size(T, H, E, K, I, Is) -> int:

@@ -278,6 +278,14 @@ int MoeRoutingGetDeviceError(int* code, void* stream);
  * into its own error word. */
 int MoeLinearGetDeviceError(int* code, void* stream);
 
+/* The kernel that MoeLinear takes for these sizes on the current device: "few", "narrow",
+ * "pairn", "wide", "pair", "split2", "split4", "split8", "split2n" or "split4n" (the names
+ * that the environment variable MOE_LINEAR_TILE takes, which forces one where it can run).
+ * NULL for sizes that MoeLinear refuses or has nothing to do for, and while MOE_LINEAR_TILE
+ * names no kernel: MoeLinear then returns MOE_ERR_UNSUPPORTED. */
+const char* MoeLinearKernel(int64_t numTokens, int64_t inFeatures, int64_t outFeatures, int outDtype,
+                            int gated);
+
 /* Synchronises `stream` and reads the device error word of a MoeExpertFFN,
  * MoeLayerForward, MoePermute or MoeEpLayerForward workspace into *code (0 = none;
  * 1 = expert id out of range; 2/4/8 = a grouped-GEMM wait timed out; expert
