@@ -236,8 +236,10 @@ constexpr int LG_THREADS = 64 + 32 * LG_EPI_WARPS;  // narrow tiles: one warp mo
 constexpr int LG_MAX_STAGES = 8;
 // The tensor cores add in fp32 but cut off instead of rounding, always towards zero: over
 // 2048 products y is 2.5e-6 of its size off (rounded sums: 0.8e-6), and in proportion over
-// more.  A 16-bit y does not show it; for an fp32 one the accumulator is emptied into
-// registers, which round, every 8 k blocks (512 products).
+// more; over products of one sign up to 2 units of 2^-24 for every 16 of them.  A 16-bit y
+// does not show it; for an fp32 one the accumulator is emptied into registers, which round,
+// every 8 k blocks (512 products), in the tiles and in the k split alike: 64 x 14336 -> 8192,
+// all positive, is then 40 units off and not 173, and takes 49.8 us and not 50.8.
 constexpr int LG_SEGMENT = 8;
 constexpr int LG_GROUP_M = 8;                  // m tiles that run together over all n tiles
 
@@ -911,7 +913,10 @@ __device__ __forceinline__ void split_finish_any(const LinParams& p, const float
         split_finish<S, BN, false, OT>(p, recv, m, col0);
 }
 
-template <int S, int BN>
+// F32: y is fp32, and every LG_SEGMENT k blocks the accumulator is emptied into registers,
+// while the next ones go to a second one.  Compiled apart from a 16-bit y, which has
+// one segment: 128 x 2048 -> 2048 takes 7.8 us so, 8.1 with both in one kernel.
+template <int S, int BN, bool F32>
 __global__ void __launch_bounds__(LS_THREADS, 1)
 linear_split_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const LinParams p)
 {
@@ -930,16 +935,16 @@ linear_split_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
     const int rank = (int)cluster_ctarank();
     const int tile = (int)(blockIdx.x / S);
     const int kb0 = (int)((long long)p.nk * rank / S), kb1 = (int)((long long)p.nk * (rank + 1) / S);
-    // an fp32 y: the sums of each `seg` k blocks have an accumulator of their own (see
-    // LG_SEGMENT; here as many as TMEM holds, added up when they are read)
-    const bool parts = p.otype == MOE_DT_FLOAT;
-    const uint32_t tmem_cols = parts ? 512 : BN;
-    const int seg = parts ? max(LG_SEGMENT, ((((kb1 - kb0) * BN + 511) / 512) + 1) & ~1) : kb1 - kb0;
+    constexpr uint32_t TMEM_COLS = F32 ? 2 * BN : BN;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < Cfg::STAGES; s++) {
             mbar_init(smem_u32(&tail->full[s]), 2);  // the copies of w, the copies of x
             mbar_init(smem_u32(&tail->empty[s]), 1);
+        }
+        if (F32) {
+            mbar_init(smem_u32(&tail->tfull[0]), 1);
+            mbar_init(smem_u32(&tail->tfull[1]), 1);
         }
         mbar_init(smem_u32(&tail->drain), 1);
         mbar_init(smem_u32(&tail->recv), 1);
@@ -950,7 +955,7 @@ linear_split_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
     }
     pdl_trigger();
     if (warp == 1) {
-        tmem_alloc(smem_u32(&tail->tmem_base), tmem_cols);
+        tmem_alloc(smem_u32(&tail->tmem_base), TMEM_COLS);
         tmem_relinquish();
     }
     int m, n;
@@ -961,7 +966,13 @@ linear_split_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
     // S slabs of 32 rows come for each of the tile's row quarters that exist
     constexpr uint32_t SLAB = 32 * PITCH * 4;
     const int quarters = min(4, (p.T - m * LG_BM + 31) / 32);
-    if (threadIdx.x == 0) mbar_arrive_expect_tx(smem_u32(&tail->recv), S * quarters * SLAB);
+    if (threadIdx.x == 0) {
+        if (F32) {
+            mbar_init(smem_u32(&tail->tempty[0]), quarters);  // one arrival per warp that reads sums
+            mbar_init(smem_u32(&tail->tempty[1]), quarters);
+        }
+        mbar_arrive_expect_tx(smem_u32(&tail->recv), S * quarters * SLAB);
+    }
     tc_fence_before();
     cluster_sync_all();  // barriers are initialised, and every CTA's shared memory is live
     tc_fence_after();
@@ -1024,9 +1035,14 @@ linear_split_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
                 if (!lin_wait<false>(smem_u32(&tail->full[s]), (it / Cfg::STAGES) & 1u, err,
                                                MOE_DEV_WAIT_TIMEOUT_MMA, abort_flag))
                     break;
+                const int part = F32 ? (kb - kb0) / LG_SEGMENT : 0, first = kb - kb0 - part * LG_SEGMENT;
+                const uint32_t acc = part & 1;
+                if (F32 && first == 0 && part >= 2 && !lin_wait<false>(smem_u32(&tail->tempty[acc]), ((part >> 1) & 1u) ^ 1u, err,
+                                                               MOE_DEV_WAIT_TIMEOUT_MMA, abort_flag))
+                    break;
                 tc_fence_after();
-                const int part = (kb - kb0) / seg, first = kb0 + part * seg;  // seg is even or the whole
-                const uint32_t d = tmem_base + part * BN;
+                const uint32_t d = tmem_base + acc * BN;
+                static_assert(LG_SEGMENT % LS_KPS == 0, "a stage belongs to one segment");
 #pragma unroll
                 for (int i = 0; i < LS_KPS; i++) {
                     if (kb + i >= kb1) break;
@@ -1035,28 +1051,49 @@ linear_split_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
 #pragma unroll
                     for (int k = 0; k < LG_BK / 16; k++)
                         umma_f16_ss(d, umma_desc_sw128(a_addr + k * 32), umma_desc_sw128(b_addr + k * 32), idesc,
-                                    (kb - first) | i | k);
+                                    first | i | k);
                 }
                 umma_commit(smem_u32(&tail->empty[s]));
+                if (F32 && (kb + LS_KPS >= kb1 || first + LS_KPS == LG_SEGMENT)) umma_commit(smem_u32(&tail->tfull[acc]));
             }
             umma_commit(smem_u32(&tail->drain));  // all sums of this CTA are in TMEM
             lin_drain<false>(smem_u32(&tail->drain), err);
         }
     } else if (warp < 6) {
         const int q = warp & 3;
-        if (q < quarters && lin_wait<false>(smem_u32(&tail->drain), 0, err, MOE_DEV_WAIT_TIMEOUT_EPI, abort_flag)) {
+        const uint32_t row = tmem_base + ((uint32_t)(q * 32) << 16);
+        const int last = F32 ? (kb1 - kb0 - 1) / LG_SEGMENT : 0;
+        float sum[F32 ? BN : 1] = {};  // of the segments before the last
+        bool got = q < quarters;
+        if constexpr (F32) {
+            for (int part = 0; got && part < last; part++) {
+                const uint32_t acc = part & 1;
+                got = lin_wait<false>(smem_u32(&tail->tfull[acc]), (part >> 1) & 1u, err, MOE_DEV_WAIT_TIMEOUT_EPI, abort_flag);
+                if (!got) break;
+                tc_fence_after();
+#pragma unroll
+                for (int j = 0; j < BN; j += 32) {
+                    float a[32];
+                    lin_tmem_load(row + acc * BN + j, a);
+#pragma unroll
+                    for (int c = 0; c < 32; c++) sum[j + c] += a[c];
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&tail->tempty[acc]));
+            }
+        }
+        if (got && lin_wait<false>(smem_u32(&tail->drain), 0, err, MOE_DEV_WAIT_TIMEOUT_EPI, abort_flag)) {
             tc_fence_after();
             // block d's row of this lane: the ring's operands have been consumed
             float* const mine = reinterpret_cast<float*>(smem) + (q * 32 + lane) * PITCH;
 #pragma unroll
             for (int j = 0; j < BN; j += 32) {
                 float a[32];
-                lin_tmem_load(tmem_base + ((uint32_t)(q * 32) << 16) + j, a);
-                for (int k0 = kb0 + seg, part = 1; k0 < kb1; k0 += seg, part++) {
-                    float more[32];
-                    lin_tmem_load(tmem_base + ((uint32_t)(q * 32) << 16) + part * BN + j, more);
+                lin_tmem_load(row + (last & 1) * BN + j, a);
+                if constexpr (F32) {
 #pragma unroll
-                    for (int c = 0; c < 32; c++) a[c] += more[c];
+                    for (int c = 0; c < 32; c++) a[c] += sum[j + c];
                 }
 #pragma unroll
                 for (int c = 0; c < 32; c += 4) {
@@ -1086,19 +1123,19 @@ linear_split_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
     const bool arrived = *abort_flag == 0;
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem_base, tmem_cols);
+        tmem_dealloc(tmem_base, TMEM_COLS);
     }
     // no CTA leaves while its sums may still be read: all have arrived here once all have
     // received
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     const int col0 = n * cols + rank * (cols / S);
     if (arrived) {
-        if (p.otype == MOE_DT_FLOAT16)
-            split_finish_any<S, BN, MOE_DT_FLOAT16>(p, recv, m, col0);
-        else if (p.otype == MOE_DT_BF16)
-            split_finish_any<S, BN, MOE_DT_BF16>(p, recv, m, col0);
-        else
+        if (F32)
             split_finish_any<S, BN, MOE_DT_FLOAT>(p, recv, m, col0);
+        else if (p.otype == MOE_DT_FLOAT16)
+            split_finish_any<S, BN, MOE_DT_FLOAT16>(p, recv, m, col0);
+        else
+            split_finish_any<S, BN, MOE_DT_BF16>(p, recv, m, col0);
     }
     __syncwarp();
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -1405,11 +1442,11 @@ cudaError_t launch_tiles(const LinearArgs& a, int dev, cudaStream_t s)
     return lin_launch(kernel, grid, Cfg::THREADS, lin_smem_bytes<PAIR, BN>(), PAIR ? 2 : 0, s, tx, tw, p);
 }
 
-template <int S, int BN>
+template <int S, int BN, bool F32>
 cudaError_t launch_split_as(const LinearArgs& a, int dev, cudaStream_t s)
 {
     static bool done[64] = {false};
-    auto* kernel = linear_split_kernel<S, BN>;
+    auto* kernel = linear_split_kernel<S, BN, F32>;
     cudaError_t e = lin_smem_attr(kernel, SplitCfg<S, BN>::SMEM, done, dev);
     if (e != cudaSuccess) return e;
     CUtensorMap tx, tw;
@@ -1423,11 +1460,12 @@ cudaError_t launch_split_as(const LinearArgs& a, int dev, cudaStream_t s)
     return lin_launch(kernel, (unsigned)(tiles * S), LS_THREADS, SplitCfg<S, BN>::SMEM, (unsigned)S, s, tx, tw, p);
 }
 
+template <bool F32>
 cudaError_t launch_split(const LinearArgs& a, int S, int bn, int dev, cudaStream_t s)
 {
-    if (S == 8) return launch_split_as<8, 128>(a, dev, s);
-    if (S == 4) return bn == 64 ? launch_split_as<4, 64>(a, dev, s) : launch_split_as<4, 128>(a, dev, s);
-    return bn == 64 ? launch_split_as<2, 64>(a, dev, s) : launch_split_as<2, 128>(a, dev, s);
+    if (S == 8) return launch_split_as<8, 128, F32>(a, dev, s);
+    if (S == 4) return bn == 64 ? launch_split_as<4, 64, F32>(a, dev, s) : launch_split_as<4, 128, F32>(a, dev, s);
+    return bn == 64 ? launch_split_as<2, 64, F32>(a, dev, s) : launch_split_as<2, 128, F32>(a, dev, s);
 }
 
 template <bool BF16, int MT, int NT>
@@ -1590,7 +1628,8 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s)
         case LIN_PAIRN: return launch_tiles<1, 128>(a, dev, s);
         case LIN_WIDE: return launch_tiles<0, 256>(a, dev, s);
         case LIN_PAIR: return launch_tiles<1, 256>(a, dev, s);
-        case LIN_SPLIT: return launch_split(a, c.S, c.bn, dev, s);
+        case LIN_SPLIT:
+            return f32 ? launch_split<true>(a, c.S, c.bn, dev, s) : launch_split<false>(a, c.S, c.bn, dev, s);
         default: return cudaErrorInvalidValue;  // MOE_LINEAR_TILE names no kernel
     }
 }
