@@ -25,6 +25,7 @@ from .ops import (  # noqa: F401
     moe_expert_ffn_workspace_size,
     moe_layer_forward,
     moe_layer_workspace_size,
+    linear_device_error,
     linear_kernel,
     moe_linear,
     moe_permute,

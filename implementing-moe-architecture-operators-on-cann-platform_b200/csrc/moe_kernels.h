@@ -134,5 +134,9 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s);
 // The kernel that launch_linear takes for these sizes, as MOE_LINEAR_TILE names it; nullptr
 // when that variable names none.
 const char* linear_kernel_name(int T, int K, int N, bool f32, bool gated);
+// Whether that kernel has waits that may give up and record in the call's error word.
+bool linear_waits(const LinearArgs& a);
+// *word = 0, in the stream's order.
+cudaError_t launch_clear_word(int* word, cudaStream_t s);
 
 }  // namespace moe

@@ -300,7 +300,7 @@ int take_error_word(int* (*find)(), int* code, void* stream)
 
 struct SharedLayout {
     LayerLayout l;
-    size_t logits, hs, total;
+    size_t logits, hs, gate_err, total;
 };
 
 SharedLayout shared_layout(int64_t T, int64_t H, int64_t E, int64_t K, int64_t I, int64_t Is)
@@ -313,6 +313,8 @@ SharedLayout shared_layout(int64_t T, int64_t H, int64_t E, int64_t K, int64_t I
     o += align_up(t * (size_t)E * 4);
     L.hs = o;
     o += align_up(t * (size_t)(Is > 0 ? Is : 1) * 2);
+    L.gate_err = o;  // what the gate records, until the permutation starts the call's error word
+    o += align_up(sizeof(int));
     L.total = o;
     return L;
 }
@@ -500,13 +502,20 @@ int MoeSharedLayerForward(const void* x, const void* w_router, const float* rout
     if (T == 0) return run_ffn(x, expert_ids, expert_weights, expert_out, T, H, E, K, I, workspace, L.l.f, s, nullptr);
     cudaEvent_t* ev = trace_begin_call();
     trace_mark(ev, 0, s);
+    // The gate's waits record in a word of this call: the library's own is that of
+    // MoeLinear calls, which may run at the same time.  (A gate that never waits, up to 16
+    // tokens, needs none.)
+    if (moe::linear_waits(gate)) {
+        gate.err = at<int>(workspace, L.gate_err);
+        rc = cuda_status(moe::launch_clear_word(gate.err, s));
+        if (rc != MOE_OK) return rc;
+    }
     rc = run_linear(gate, s);
     if (rc == MOE_OK) rc = cuda_status(moe::launch_select(sel, MOE_DT_FLOAT, s));
     if (rc != MOE_OK) return rc;
     trace_mark(ev, 1, s);
     // the permutation clears the call's error word, or sets it to what the gate recorded
-    rc = run_ffn(x, expert_ids, expert_weights, expert_out, T, H, E, K, I, workspace, L.l.f, s, ev,
-                 moe::linear_error_word());
+    rc = run_ffn(x, expert_ids, expert_weights, expert_out, T, H, E, K, I, workspace, L.l.f, s, ev, gate.err);
     up.err = down.err = at<int>(workspace, L.l.f.p.err);
     // the shared expert reads x before the combine writes y, which may be x
     if (rc == MOE_OK && Is > 0) rc = run_linear(up, s);

@@ -392,6 +392,21 @@ def moe_linear(x, weight, bias=None, activation: str = "none", gated: bool = Fal
     return y
 
 
+def linear_device_error(device=None) -> int:
+    """Reads and clears the error word of the moe_linear calls on `device` (default: the
+    current one; synchronises its current stream).  0, or 2/4/8 where a wait gave up and y is
+    not complete: never expected.  Concurrent calls on one device share the word."""
+    torch = _torch()
+    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    if dev.type != "cuda":
+        raise MoeError(-1, f"device must be a CUDA device, got {dev}")
+    if dev.index is None:
+        dev = torch.device("cuda", torch.cuda.current_device())
+    code = ctypes.c_int(0)
+    _check(_call_on(dev, lib().MoeLinearGetDeviceError, ctypes.byref(code)), "MoeLinearGetDeviceError")
+    return code.value
+
+
 def linear_kernel(T: int, K: int, N: int, out_dtype=None, gated: bool = False):
     """The name of the kernel that moe_linear takes for x [T,K] and y [T,N] on the current
     device (out_dtype float32 or, by default, 16 bits): a value of MOE_LINEAR_TILE, or None

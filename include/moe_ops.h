@@ -274,8 +274,9 @@ int MoeRoutingGetDeviceError(int* code, void* stream);
 
 /* The same for MoeLinear, which has no workspace either: synchronises `stream`, writes
  * the word its bounded waits record into (2/4/8 = a copy, tensor-core or epilogue wait
- * gave up; never expected) to *code and clears it.  MoeSharedLayerForward moves the word
- * into its own error word. */
+ * gave up; never expected) to *code and clears it.  y of such a call is not complete.
+ * Concurrent MoeLinear calls on one device share the word; MoeSharedLayerForward records
+ * in its workspace instead. */
 int MoeLinearGetDeviceError(int* code, void* stream);
 
 /* The kernel that MoeLinear takes for these sizes on the current device: "few", "narrow",
@@ -287,8 +288,9 @@ const char* MoeLinearKernel(int64_t numTokens, int64_t inFeatures, int64_t outFe
                             int gated);
 
 /* Synchronises `stream` and reads the device error word of a MoeExpertFFN,
- * MoeLayerForward, MoePermute or MoeEpLayerForward workspace into *code (0 = none;
- * 1 = expert id out of range; 2/4/8 = a grouped-GEMM wait timed out; expert
+ * MoeLayerForward, MoeSharedLayerForward, MoePermute or MoeEpLayerForward workspace into
+ * *code (0 = none; 1 = expert id out of range; 2/4/8 = a grouped-GEMM wait, or one of the
+ * gate or the shared expert, timed out; expert
  * parallel: 64/128/256 = the counts / rows / returned-rows flag wait timed out,
  * 512 = more rows than the workspace's maxRecvRows).  Returns MOE_OK or
  * MOE_ERR_CUDA. */
@@ -296,13 +298,15 @@ int MoeGetDeviceError(const void* workspace, int* code, void* stream);
 
 /* Stage tracing (the profiling hook of this library; the reference only has
  * host wall-clock timers, tests/test_moe.cpp:592-605).  Between MoeTraceStart
- * and MoeTraceStop, every MoeLayerForward / MoeExpertFFN call made on this host
- * thread records CUDA events at its stage boundaries on its stream, for up to
+ * and MoeTraceStop, every MoeLayerForward / MoeSharedLayerForward / MoeExpertFFN call
+ * made on this host thread records CUDA events at its stage boundaries on its stream, for up to
  * maxCalls calls.  MoeTraceStop synchronises on those events and writes, per
  * call, MOE_TRACE_STAGES durations in milliseconds (routing, permute, gather (in
  * MoeEpLayerForward: gather, count exchange, dispatch and reorder),
  * gate/up GEMM + SwiGLU, down GEMM, combine (with the EP return exchange); stages a
- * call does not run read 0).  MoeEpLayerForward calls are traced too. */
+ * call does not run read 0).  MoeEpLayerForward calls are traced too.  In
+ * MoeSharedLayerForward routing is the gate and the selection, and combine has the shared
+ * expert with it. */
 #define MOE_TRACE_STAGES 6
 int MoeTraceStart(int maxCalls);
 int MoeTraceStop(float* stageMs, int maxCalls, int* numCalls);
