@@ -41,9 +41,14 @@ namespace moe {
 __device__ int g_linear_err;
 
 // ---------------------------------------------------------------------- epilogue maths
-// exp and the quotient by their fast intrinsics: together below 8 + 2|z| half ulps, which
-// the fp16 / bf16 rounding of y hides, and of the size of the sum's own roundings for an
-// fp32 y.  Results below about 2^-126 become 0.
+// exp and the quotient by their fast intrinsics.  __expf(a) is off by up to 2 + 1.173 |a| ulp
+// and carries what a itself is off, so a result is off by, in units of 2^-24 of itself,
+//   SiLU, sigmoid   10 + 2.4 |z|                              (a = -z is exact)
+//   GELU            28 + 1.7 z^2                              (a = P - z^2 / 2, rounded once)
+//   GELU, tanh      9 + 9.4 |u|, u = 1.6 (z + 0.0447 z^3)     (a = -u, seven roundings)
+// at most.  An fp16 or bf16 y (half a step: 2^13 or 2^16 units) hides that until a result is
+// far below its normal range; of an fp32 y it is the accuracy.  A quotient by more than
+// 2^126 is 0: results below |z| 2^-126 (sigmoid: 2^-126) may become 0.
 template <int ACT>
 __device__ __forceinline__ float lin_act1(float z)
 {

@@ -159,7 +159,8 @@ int MoeRouterSelect(const void* logits, int logitsDtype, int64_t ldLogits, const
  *               Wu [N, K], bias = bg [N] then bu [N]
  * x [T, K], W and bias have the type dtype (MOE_DT_FLOAT16 or MOE_DT_BF16); y [T, N]
  * and residual [T, N] the type outDtype (dtype, or MOE_DT_FLOAT).  bias and residual
- * may be NULL.  Sums and the epilogue are fp32; y is rounded once.  ldx, ldw, ldr, ldy:
+ * may be NULL.  Sums and the epilogue are fp32; y is rounded once.  An activation of z
+ * that lies within |z| 2^-126 (sigmoid: 2^-126) of 0 may become 0.  ldx, ldw, ldr, ldy:
  * elements from one row to the next (0: contiguous).  K, ldx and ldw are multiples of
  * 8 and x and W 16-byte aligned; N, ldr, ldy and the other pointers are free (best when
  * 16-byte aligned too).  residual may be y itself (same rows); y overlaps no other
