@@ -14,8 +14,9 @@
 // order, with weight 0.
 //
 // The choice is that of keys in 64 bits: two scores may lie closer together than 32
-// bits tell apart, and the id is a whole number that is right or wrong.  Without a bias
-// scores order as their logits do, so the logits themselves are the keys.
+// bits tell apart, and the id is a whole number that is right or wrong.  Scores order as
+// their logits do, so where nothing is added to them (no bias, and one group or groupTop 1)
+// the logits themselves are the keys.
 //
 // Measured, 65536 x 256 fp32 logits, sigmoid, bias, 4 of 8 groups, K = 8: 50 us, 1.4 TB/s.  It
 // reads its 67 MB once; what bounds it is the ALU pipe, on which a min or max takes two issue

@@ -133,8 +133,10 @@ int MoeLayerForward(const void* x, const void* w_gate, const void* expert_weight
  *   ids    the topK largest keys, larger first, ties to the lower id;
  *   weight s of the chosen expert, divided by the sum over the topK when renormalize
  *          is nonzero, times scale.
- * The choice is exact: keys that differ in 64-bit arithmetic are told apart (without a
- * bias, logits that differ at all).  An expert whose logit or bias is -inf or NaN, or
+ * The choice is exact: keys that differ in 64-bit arithmetic are told apart.  Where no
+ * score is added to anything (no bias, and one group or groupTop 1) the logits take the
+ * scores' place and are told apart where they differ at all; sigmoids of 40 and 41 are the
+ * same in 64 bits, and then tie.  An expert whose logit or bias is -inf or NaN, or
  * whose group did not stay, is closed: it is chosen only when no open expert is left,
  * lowest id first, and then has weight 0.  A +inf logit has score 1 (softmax: +inf
  * logits share it).
