@@ -19,7 +19,7 @@
 //       registers of mma.sync fragments; bound by HBM (by latency for small w).
 // Measured, cold L2, the kernel alone, against the 6515 GB/s of a copy and the 1679 TFLOP/s of
 // a library product: few 8 x 8192 -> 2048 with residual 9.2 us (3.7 TB/s; 128 blocks on 148
-// SMs), split 128 x 2048 -> 2048 8.0 us (latency of the first copies and of the exchange), gemm
+// SMs), split 128 x 2048 -> 2048 7.8 us (latency of the first copies and of the exchange), gemm
 // 128 x 2048 -> 8192 gated 15.1 us (4.6 TB/s), 4096 x 8192 -> 2048 102 us (1351 TFLOP/s; 128
 // tiles on 74 pairs), 8192 x 4096 -> 14336 gated 1229 us (1565 TFLOP/s; tensor pipe, 92% busy
 // on a smaller shape).
@@ -1513,8 +1513,8 @@ cudaError_t launch_few(const LinearArgs& a, int sms, cudaStream_t s)
 // the exchange of partial sums 800 and its bytes at 21 per ns, the rate measured for
 // distributed shared memory.  `cap` is how many CTAs run at once: a cluster of 8 (4, 2)
 // finds room 15 (33, 74) times.  Against the measured order: 128 x 2048 -> 2048: <4, 64>
-// 8.2 us, <4, 128> 10.5, <2, 64> 9.7, whole tiles 11.1; 17 x 7168 -> 256: <8, 128> 8.3,
-// <4, 64> 10.9; 512 x 2048 -> 2048: whole tiles 11.3, <2, 128> 13.4.
+// 7.9 us, <2, 64> 8.6, <4, 128> 10.3, whole tiles 11.1; 17 x 7168 -> 256: <8, 128> 8.3,
+// <4, 64> 8.7, <4, 128> 12.2; 512 x 2048 -> 2048: whole tiles 11.5, <2, 128> 13.4.
 struct SplitChoice {
     int S, bn;
 };

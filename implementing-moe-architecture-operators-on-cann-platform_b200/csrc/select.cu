@@ -19,8 +19,11 @@
 // the logits themselves are the keys.
 //
 // Measured, 65536 x 256 fp32 logits, sigmoid, bias, 4 of 8 groups, K = 8: 50 us, 1.4 TB/s.  It
-// reads its 67 MB once; what bounds it is the ALU pipe, on which a min or max takes two issue
-// cycles: 422 instructions per token, 207 of them there, issue slots 61% used.
+// reads its 67 MB once.  No unit is full: 422 instructions per token take 61% of the issue
+// slots, and the 207 of them on the ALU pipe (where a min or max takes two cycles) 57% of it.
+// What bounds it is latency with few warps: 96 registers leave 4.5 per scheduler, of which at
+// each issue 2.1 wait for a result of fixed latency, 1.2 for shared memory, a shuffle or a
+// special function, and 0.7 for the pipe.
 #include <math_constants.h>
 
 #include <cuda_bf16.h>
